@@ -40,6 +40,8 @@ EXPORTED = [
     "ca_scaled_norm", "ca_clamped_glu", "ca_softcap", "ca_latent_store", "ca_latent_block", "ca_latent_attention", "ca_latent_decodes", "ca_latent_gather",
     "ca_latent_expands", "ca_latent_expanded_block", "ca_latent_expanded",
     "ca_plan_build_windowed", "ca_plan_direct",
+    "ca_draft_plan_build", "ca_draft_plan_for_context", "ca_draft_plan_data", "ca_draft_plan_destroy", "ca_draft_partial_floats", "ca_draft_attention",
+    "ca_accept_draft", "ca_log_probs_scratch", "ca_token_log_probs",
 ]
 CA_STATIC_MAX_SLOTS = 16384
 
@@ -57,6 +59,12 @@ class PlanStats(C.Structure):
 
     def as_dict(self):
         return {f: getattr(self, f) for f, _ in self._fields_}
+
+
+class DraftPlanInfo(C.Structure):
+    _fields_ = [("n_items", C.c_int32), ("n_merge", C.c_int32), ("n_slots", C.c_int32), ("n_nodes", C.c_int32), ("block_rows", C.c_int32),
+                ("longest", C.c_int32), ("n_data", C.c_int64), ("at_tiles", C.c_int64), ("at_nodes", C.c_int64), ("at_off", C.c_int64),
+                ("at_slots", C.c_int64)]
 
 
 class CAError(RuntimeError):
@@ -103,6 +111,10 @@ def _load():
         "ca_plan_array": (i32, [vp, i32, C.POINTER(C.POINTER(C.c_int32)), C.POINTER(i64)]),
         "ca_plan_stats_get": (i32, [vp, C.POINTER(PlanStats)]),
         "ca_plan_destroy": (None, [vp]),
+        "ca_draft_plan_build": (i32, [C.POINTER(vp), C.POINTER(ChunkInfo), i32, C.POINTER(C.c_int32), i32, i32, i32, i64, i32, i32, i32, i32]),
+        "ca_draft_plan_data": (i32, [vp, C.POINTER(C.POINTER(C.c_int32)), C.POINTER(DraftPlanInfo)]),
+        "ca_draft_plan_destroy": (None, [vp]),
+        "ca_log_probs_scratch": (i64, [i32, i32, i32, i32]),
         "ca_rms_norm": (i32, [vp, vp, vp, C.c_float, i64, i32, i32, vp]),
         "ca_fused_add_rms_norm": (i32, [vp, vp, vp, C.c_float, i64, i32, i32, vp]),
         "ca_rotary_embedding": (i32, [vp, vp, vp, vp, i32, i64, i64, i32, i32, i32, i64, i32, i32, i64, vp, vp]),
@@ -185,6 +197,32 @@ class Plan:
     def __del__(self):
         if getattr(self, "_h", None):
             lib.ca_plan_destroy(self._h)
+            self._h = None
+
+
+class DraftPlan:
+    """The work list of attention over drafted trees (host-only): first[0 .. n_rows] is the first node of every row's tree."""
+
+    def __init__(self, infos, first, chunk_size=64, tpp_threshold=1, max_chunks=1 << 30, kv_heads=1, group=1, block_rows=128, ctas=296):
+        arr, n = make_infos(infos)
+        self._h = C.c_void_p()
+        f = (C.c_int32 * len(first))(*first)
+        check(lib.ca_draft_plan_build(C.byref(self._h), arr, n, f, len(first) - 1, chunk_size, tpp_threshold, max_chunks, kv_heads, group, block_rows, ctas))
+        self.info = DraftPlanInfo()
+        ptr = C.POINTER(C.c_int32)()
+        check(lib.ca_draft_plan_data(self._h, C.byref(ptr), C.byref(self.info)))
+        i = self.info
+        data = np.ctypeslib.as_array(ptr, shape=(i.n_data,)).copy() if i.n_data else np.zeros(0, np.int32)
+        # items: first node, nodes, list, tiles, slot, first node of the tree, drafted nodes seen, tokens
+        self.items = data[:8 * i.n_items].reshape(-1, 8)
+        self.tiles = data[i.at_tiles:i.at_nodes]
+        self.merge_nodes = data[i.at_nodes:i.at_nodes + i.n_merge]
+        self.merge_off = data[i.at_off:i.at_off + i.n_merge + 1]
+        self.merge_slots = data[i.at_slots:]
+
+    def __del__(self):
+        if getattr(self, "_h", None):
+            lib.ca_draft_plan_destroy(self._h)
             self._h = None
 
 

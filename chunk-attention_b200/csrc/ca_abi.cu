@@ -6,11 +6,15 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <exception>
+#include <memory>
 #include <new>
 #include <string>
 
 #include "../../include/chunk_attn_b200.h"
+#include "ca_draft.h"
 #include "ca_kernels.h"
+#include "ca_logits.h"
 #include "ca_plan.h"
 
 namespace {
@@ -84,6 +88,11 @@ struct ca_plan {
     int d_head = ca::FAST_D;
     int esize = 2;
     int window = 0, group = 1;
+};
+
+struct ca_draft_plan {
+    ca::DraftPlan plan;
+    int block_rows = 0;
 };
 
 namespace {
@@ -1692,5 +1701,209 @@ int ca_plan_stats_get(const ca_plan* plan, ca_plan_stats* out) {
 }
 
 void ca_plan_destroy(ca_plan* plan) { delete plan; }
+
+// ---- drafted tokens ------------------------------------------------------------------------------------------------------------
+static int make_draft_plan(ca_draft_plan** out, const ca_chunk_info* infos, int n_infos, const int32_t* first, int n_rows, const ca::DraftPlanShape& shape) {
+    *out = nullptr;
+    try {
+        std::unique_ptr<ca_draft_plan> p(new ca_draft_plan);
+        const std::string err = ca::build_draft_plan(p->plan, infos, n_infos, first, n_rows, shape);
+        if (!err.empty()) return fail(CA_ERR_INVALID, err);
+        p->block_rows = shape.block_rows;
+        *out = p.release();
+    } catch (const std::exception& e) {
+        return fail(CA_ERR_INVALID, std::string("draft plan: ") + e.what());
+    }
+    return CA_OK;
+}
+
+int ca_draft_plan_build(ca_draft_plan** out, const ca_chunk_info* infos, int n_infos, const int32_t* first, int n_rows, int chunk_size,
+                        int tpp_threshold, int64_t max_chunks, int kv_heads, int group, int block_rows, int ctas) {
+    if (!out) return fail(CA_ERR_INVALID, "null argument");
+    ca::DraftPlanShape shape;
+    shape.chunk_size = chunk_size;
+    shape.tpp_threshold = tpp_threshold;
+    shape.max_chunks = max_chunks;
+    shape.kv_heads = kv_heads;
+    shape.group = group;
+    shape.block_rows = block_rows;
+    shape.ctas = ctas;
+    return make_draft_plan(out, infos, n_infos, first, n_rows, shape);
+}
+
+int ca_draft_plan_for_context(const ca_context* c, ca_draft_plan** out, const ca_chunk_info* infos, int n_infos, const int32_t* first, int n_rows) {
+    if (!c || !out || !first || n_rows < 0) return fail(CA_ERR_INVALID, "null or negative argument");
+    if (c->shape.latent) return fail(CA_ERR_INVALID, "drafted tokens: a latent cache is not served");
+    int most = 0;
+    for (int r = 0; r < n_rows; r++) {
+        if (first[r + 1] - first[r] > CA_DRAFT_MAX_NODES) return fail(CA_ERR_INVALID, "drafted tokens: a tree has too many nodes");
+        most = std::max(most, first[r + 1] - first[r]);
+    }
+    ca::DraftPlanShape shape;
+    shape.chunk_size = c->geo.chunk_size;
+    shape.tpp_threshold = c->tpp_threshold;
+    shape.max_chunks = c->max_chunks;
+    shape.kv_heads = c->geo.n_heads;
+    shape.group = c->group;
+    // A run that rows share has the nodes of them all
+    int widest = most;
+    for (int i = 0; i < n_infos; i++)
+        if (infos && infos[i].n_tokens > 0 && infos[i].seq_begin >= 0 && infos[i].seq_end <= n_rows && infos[i].seq_end - infos[i].seq_begin > c->tpp_threshold)
+            widest = std::max(widest, first[infos[i].seq_end] - first[infos[i].seq_begin]);
+    shape.block_rows = ca::draft_generic_rows(std::min(widest, 64) * c->group);
+    shape.ctas = 4 * ca::B200_SMS;
+    if (c->group > shape.block_rows) return fail(CA_ERR_INVALID, "drafted tokens: more than 64 query heads to a key/value head");
+    return make_draft_plan(out, infos, n_infos, first, n_rows, shape);
+}
+
+int ca_draft_plan_data(const ca_draft_plan* p, const int32_t** data, ca_draft_plan_info* info) {
+    if (!p || !data || !info) return fail(CA_ERR_INVALID, "null argument");
+    const ca::DraftPlan& pl = p->plan;
+    *data = pl.data.data();
+    info->n_items = (int32_t)pl.items.size();
+    info->n_merge = (int32_t)pl.merge_nodes.size();
+    info->n_slots = pl.n_slots;
+    info->n_nodes = pl.n_nodes;
+    info->block_rows = p->block_rows;
+    info->longest = pl.items.empty() ? 0 : pl.items.front().tokens + pl.items.front().n_drafted;
+    info->n_data = (int64_t)pl.data.size();
+    info->at_tiles = pl.at_tiles;
+    info->at_nodes = pl.at_nodes;
+    info->at_off = pl.at_off;
+    info->at_slots = pl.at_slots;
+    return CA_OK;
+}
+
+void ca_draft_plan_destroy(ca_draft_plan* p) { delete p; }
+
+static int draft_part_width(const ca_context* c) { return (c->geo.d_value + 3) / 4 * 4; }
+
+int64_t ca_draft_partial_floats(const ca_context* c, const ca_draft_plan_info* info) {
+    if (!c || !info || info->n_slots < 0) return -1;
+    const int64_t pairs = (int64_t)info->n_slots * c->geo.n_heads * c->group;
+    return 2 * ((pairs + 1) / 2 * 2) + pairs * draft_part_width(c);
+}
+
+int ca_draft_attention(ca_context* c, const ca_draft_args* a, ca_stream stream_) {
+    if (!c || !a || !a->info) return fail(CA_ERR_INVALID, "null argument");
+    if (c->shape.latent) return fail(CA_ERR_INVALID, "drafted tokens: a latent cache is not served");
+    if (a->info->n_nodes <= 0 || a->info->n_items <= 0) return a->info->n_nodes == 0 ? CA_OK : fail(CA_ERR_INVALID, "drafted tokens: bad work list");
+    if (!a->q || !a->k || !a->v || !a->out || !a->seen || !a->work) return fail(CA_ERR_INVALID, "drafted tokens: null operand");
+    if (a->words < 2 || a->words > CA_DRAFT_MAX_NODES / 32 || a->words % 2) return fail(CA_ERR_INVALID, "drafted tokens: words must be even, 2 to 8");
+    if (a->info->n_slots > 0 && !a->partials) return fail(CA_ERR_INVALID, "drafted tokens: no room for partial results");
+    if (reinterpret_cast<uintptr_t>(a->out) % 16 || reinterpret_cast<uintptr_t>(a->work) % 16 || reinterpret_cast<uintptr_t>(a->seen) % 8 ||
+        reinterpret_cast<uintptr_t>(a->partials) % 16)
+        return fail(CA_ERR_INVALID, "drafted tokens: out, work list and scratch must be 16-byte aligned");
+    if ((int64_t)a->info->n_items * c->geo.n_heads > INT32_MAX) return fail(CA_ERR_INVALID, "drafted tokens: too many pieces of work");
+    DeviceGuard guard(c->device);
+    if (guard.err != cudaSuccess) return fail_cuda(guard.err, "cudaSetDevice");
+    const int H = c->geo.n_heads * c->group;
+    ca::DraftParams p{};
+    p.pool = c->pool;
+    p.geo = c->geo;
+    p.group = c->group;
+    p.d_key = c->shaped ? c->shape.d_key : c->geo.d_head;
+    p.d_value = c->shaped ? c->shape.d_value : c->geo.d_head;
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.q_node = a->q_node;
+    p.q_head = a->q_head;
+    p.k_node = a->k_node;
+    p.k_head = a->k_head;
+    p.v_node = a->v_node;
+    p.v_head = a->v_head;
+    p.out = a->out;
+    p.scale_log2 = (c->shaped ? c->shape.scale : 1.f / std::sqrt((float)c->geo.d_head)) * 1.4426950408889634f;
+    p.sink = c->shaped ? c->shape.sink : 0;
+    p.seen = a->seen;
+    p.words = a->words;
+    p.items = reinterpret_cast<const ca::DraftItem*>(a->work);
+    p.n_items = a->info->n_items;
+    p.n_nodes = a->info->n_nodes;
+    p.tiles = a->work + a->info->at_tiles;
+    p.part_width = draft_part_width(c);
+    p.part_ml = reinterpret_cast<float2*>(a->partials);
+    p.part_o = a->partials + 2 * (((int64_t)a->info->n_slots * H + 1) / 2 * 2);
+    p.merge_nodes = a->work + a->info->at_nodes;
+    p.merge_off = a->work + a->info->at_off;
+    p.merge_slots = a->work + a->info->at_slots;
+    p.n_merge = a->info->n_merge;
+    p.max_chunks = (int)c->max_chunks;
+    p.status = c->status;
+    p.wait_limit = c->opt_wait_limit;
+    p.dependent = c->opt_pdl;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    CA_CUDA(ca::launch_draft_generic(p, a->info->block_rows, c->dtype, stream));
+    CA_CUDA(ca::launch_draft_merge(p, c->dtype, stream));
+    return CA_OK;
+}
+
+int ca_accept_draft(const ca_accept_args* a, ca_stream stream) {
+    if (!a) return fail(CA_ERR_INVALID, "null argument");
+    if (a->n_rows < 0 || a->width < 0) return fail(CA_ERR_INVALID, "accept_draft: negative size");
+    if (a->n_rows == 0) return CA_OK;
+    if (!a->first || !a->parent || !a->depth || !a->seen || !a->tokens || !a->choice || !a->count || !a->next || (a->width > 0 && !a->path))
+        return fail(CA_ERR_INVALID, "accept_draft: null operand");
+    if (a->words < 1 || a->words > CA_DRAFT_MAX_NODES / 32) return fail(CA_ERR_INVALID, "accept_draft: words must be 1 to 8");
+    if ((a->log_probs == nullptr) != (a->entropy == nullptr)) return fail(CA_ERR_INVALID, "accept_draft: log_probs and entropy come together");
+    if (a->log_probs && !(a->epsilon > 0 && a->delta > 0)) return fail(CA_ERR_INVALID, "accept_draft: epsilon and delta must be positive");
+    ca::AcceptParams p{};
+    p.first = a->first;
+    p.parent = a->parent;
+    p.depth = a->depth;
+    p.seen = a->seen;
+    p.words = a->words;
+    p.n_rows = a->n_rows;
+    p.width = a->width;
+    p.tokens = a->tokens;
+    p.choice = a->choice;
+    p.log_probs = a->log_probs;
+    p.entropy = a->entropy;
+    if (a->log_probs) {
+        p.log_epsilon = (float)std::log(a->epsilon);
+        p.log_delta = (float)std::log(a->delta);
+    }
+    p.path = a->path;
+    p.count = a->count;
+    p.next = a->next;
+    CA_CUDA(ca::launch_accept_draft(p, static_cast<cudaStream_t>(stream)));
+    return CA_OK;
+}
+
+// ---- log probabilities ---------------------------------------------------------------------------------------------------------
+int64_t ca_log_probs_scratch(int n_rows, int vocab, int dtype, int top) {
+    if (n_rows < 0 || vocab < 1 || top < 0 || top > CA_MAX_TOP || !shaped_esize_of(dtype)) return -1;
+    return (int64_t)n_rows * sizeof(float2);
+}
+
+int ca_token_log_probs(const ca_log_probs_args* a, ca_stream stream) {
+    if (!a) return fail(CA_ERR_INVALID, "null argument");
+    if (a->n_rows < 0 || a->n_tokens < 0 || a->vocab < 1) return fail(CA_ERR_INVALID, "token_log_probs: bad sizes");
+    if (!shaped_esize_of(a->dtype)) return fail(CA_ERR_INVALID, "token_log_probs: fp16, bf16 and fp32 only");
+    if (a->top < 0 || a->top > CA_MAX_TOP || a->top > a->vocab) return fail(CA_ERR_INVALID, "token_log_probs: top must be 0 to 32 and not above the vocabulary");
+    if (a->row_stride < 0) return fail(CA_ERR_INVALID, "token_log_probs: negative stride");
+    if (a->n_rows > 0 && (!a->logits || !a->entropy || !a->scratch)) return fail(CA_ERR_INVALID, "token_log_probs: null operand");
+    if (a->n_tokens > 0 && (!a->tokens || !a->log_probs)) return fail(CA_ERR_INVALID, "token_log_probs: null operand");
+    if (a->n_rows > 0 && a->top > 0 && (!a->top_ids || !a->top_log_probs)) return fail(CA_ERR_INVALID, "token_log_probs: null operand");
+    ca::LogProbsParams p{};
+    p.logits = a->logits;
+    p.row_stride = a->row_stride;
+    p.n_rows = a->n_rows;
+    p.vocab = a->vocab;
+    p.splits = ca::log_probs_splits(a->n_rows, a->vocab);
+    if ((int64_t)p.n_rows * p.splits > INT32_MAX) return fail(CA_ERR_INVALID, "token_log_probs: too many rows");
+    p.tokens = a->tokens;
+    p.rows = a->rows;
+    p.n_tokens = a->n_tokens;
+    p.top = a->top;
+    p.log_probs = a->log_probs;
+    p.entropy = a->entropy;
+    p.top_log_probs = a->top_log_probs;
+    p.top_ids = a->top_ids;
+    p.lse = static_cast<float2*>(a->scratch);
+    CA_CUDA(ca::launch_log_probs(p, a->dtype, static_cast<cudaStream_t>(stream)));
+    return CA_OK;
+}
 
 }  // extern "C"

@@ -33,6 +33,7 @@ Attention::Attention(Attention& other)
     options_(other.options_) {
     init();
     shared_plan_ = other.shared_plan_;  // same configuration, same sequence of tree operations: same work lists
+    shared_draft_ = other.shared_draft_;
     shared_tables_ = other.shared_tables_;
 }
 
@@ -111,6 +112,7 @@ void Attention::init() {
     valid_ = false;
     shared_plan_ = std::make_shared<SharedPlan>();
     shared_tables_ = std::make_shared<SharedTables>();
+    shared_draft_ = std::make_shared<std::shared_ptr<DraftWork>>();
 }
 
 Attention::SharedPlan::~SharedPlan() {
@@ -565,6 +567,114 @@ torch::Tensor Attention::forward_rows(torch::Tensor q, torch::Tensor positions, 
     }
     check_rc(ca_attention_rows(ctx_, &a, stream()), "forward_rows");
     return out;
+}
+
+// ---- drafted tokens -----------------------------------------------------------------------------------------------------
+
+namespace {
+struct DraftPlanHandle {
+    ca_draft_plan* plan = nullptr;
+    ~DraftPlanHandle() {
+        if (plan) ca_draft_plan_destroy(plan);
+    }
+};
+}  // namespace
+
+torch::Tensor Attention::forward_draft(torch::Tensor q, torch::Tensor k, torch::Tensor v, DraftBatch& draft) {
+    if (shape_.latent) throw std::runtime_error("forward_draft: a latent cache is not served");
+    const auto st = c10::typeMetaToScalarType(options_.dtype());
+    const int64_t n = draft.n_nodes(), dv = shaped_ ? shape_.d_value : d_head_;
+    if (draft.n_rows() != tree_->n_seqs()) throw std::runtime_error("forward_draft: one tree per live sequence is required");
+    if (draft.device() != options_.device()) throw std::runtime_error("forward_draft: the draft is on another device than the cache");
+    auto fits = [&](const torch::Tensor& t, int64_t heads, int64_t d) {
+        return t.dim() == 3 && t.size(0) == n && t.size(1) == heads && t.size(2) == d && (t.stride(2) == 1 || d == 1) && t.device() == options_.device() &&
+               t.scalar_type() == st;
+    };
+    if (!fits(q, n_heads_, d_head_) || !fits(k, kv_heads(), d_head_) || !fits(v, kv_heads(), dv))
+        throw std::runtime_error("forward_draft: q must be [n_nodes, n_heads, d_key], k and v [n_nodes, n_kv_heads, .] with the dtype and device of the cache and contiguous heads");
+    c10::cuda::CUDAGuard guard(options_.device());
+    torch::Tensor out = torch::empty({n, n_heads_, dv}, options_);
+    if (n == 0) return out;
+    if (!draft_ || draft_->serial != draft.serial() || draft_version_ != tree_->version() || draft_appended_ != tree_->appended()) {
+        std::vector<ca_chunk_info> infos = tree_->get_chunks();
+        std::shared_ptr<DraftWork>& shared = *shared_draft_;
+        const bool same = shared && shared->serial == draft.serial() && shared->infos.size() == infos.size() &&
+                          (infos.empty() || std::memcmp(shared->infos.data(), infos.data(), infos.size() * sizeof(ca_chunk_info)) == 0);
+        if (!same) {
+            DraftPlanHandle h;
+            check_rc(ca_draft_plan_for_context(ctx_, &h.plan, infos.data(), (int)infos.size(), draft.first().data(), draft.n_rows()), "forward_draft");
+            auto work = std::make_shared<DraftWork>();
+            const int32_t* data = nullptr;
+            check_rc(ca_draft_plan_data(h.plan, &data, &work->info), "forward_draft");
+            work->device = Uploaded(std::vector<int32_t>(data, data + work->info.n_data), options_.device(), "forward_draft");
+            work->serial = draft.serial();
+            work->infos.swap(infos);
+            shared = work;
+        }
+        draft_ = shared;
+        draft_version_ = tree_->version();
+        draft_appended_ = tree_->appended();
+    }
+    ca_draft_args a{};
+    a.q = q.data_ptr();
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    a.q_node = q.stride(0);
+    a.q_head = q.stride(1);
+    a.k_node = k.stride(0);
+    a.k_head = k.stride(1);
+    a.v_node = v.stride(0);
+    a.v_head = v.stride(1);
+    a.out = out.data_ptr();
+    a.seen = draft.view(&captured_).seen;
+    a.words = draft.words();
+    a.work = draft_->device.use();
+    a.info = &draft_->info;
+    if (capturing(options_.device())) captured_.push_back(draft_->device.tensor());  // a replay reads it, whatever the tree has become
+    torch::Tensor scratch;
+    const int64_t floats = ca_draft_partial_floats(ctx_, a.info);
+    if (floats > 0) {
+        scratch = torch::empty({floats}, options_.dtype(torch::kFloat32));
+        a.partials = scratch.data_ptr<float>();
+    }
+    check_rc(ca_draft_attention(ctx_, &a, stream()), "forward_draft");
+    return out;
+}
+
+void Attention::extend_kv(const std::vector<int>& rows, const std::vector<std::vector<int>>& tokens, torch::Tensor k, torch::Tensor v) {
+    need_owner();
+    const size_t n = rows.size();
+    if (tokens.size() != n) throw std::runtime_error("extend_kv: one token list per row is required");
+    // everything that can be refused is refused before anything changes
+    std::vector<char> seen(tree_->n_seqs(), 0);
+    int64_t need = 0, total = 0;
+    for (size_t i = 0; i < n; i++) {
+        need += tree_->extend_need(rows[i], (int)tokens[i].size());
+        if (seen[rows[i]]++) throw std::runtime_error("extend_kv: a row is named twice");
+        total += (int64_t)tokens[i].size();
+    }
+    check_kv(k, v, total, "extend_kv: k and v must be [n_tokens, n_heads, d_head]");
+    if (tree_->pool().max_chunks() - tree_->pool().in_use() < need) throw std::runtime_error("ChunkAllocator: capacity reached");
+    if (total == 0) return;
+    k = pad_heads(to_cache(k), k_padded_);
+    v = pad_heads(to_cache(v), v_padded_);
+    if (k.strides() != v.strides() || k_padded_ != v_padded_) {
+        k = k.contiguous();
+        v = v.contiguous();
+    }
+    valid_ = false;
+    tables_->n_tokens = -1;
+    std::vector<int32_t> ids, at;
+    for (size_t i = 0; i < n; i++) {
+        std::vector<std::pair<Chunk*, int>> slots;
+        tree_->extend_seq(rows[i], tokens[i], slots);
+        for (const auto& s : slots) {
+            ids.push_back(s.first->id);
+            at.push_back(s.second);
+        }
+    }
+    c10::cuda::CUDAGuard guard(options_.device());
+    check_rc(ca_scatter_rows(ctx_, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), (int)ids.size(), ids.data(), at.data(), stream()), "extend_kv");
 }
 
 // ---- latent caches ------------------------------------------------------------------------------------------------------

@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "../../../include/chunk_attn_b200.h"
+#include "draft.h"
 #include "prefix_tree.h"
 
 namespace ca_host {
@@ -63,6 +64,14 @@ class Attention {
     // [n_rows, n_heads, d_value]: decode over every row (row_entry not given), or the tokens of the last extend
     torch::Tensor forward_rows(torch::Tensor q, torch::Tensor positions, c10::optional<torch::Tensor> value_freq,
                                c10::optional<torch::Tensor> row_entry);
+    // ---- drafted tokens ----
+    // Every row's tree of drafted tokens: node i attends to the cached tokens of its row, its ancestors and itself.  q [n_nodes,
+    // n_heads, d_key], k [n_nodes, n_kv_heads, d_key], v [n_nodes, n_kv_heads, d_value], as they would be stored (rotated and so on); nothing
+    // is added to the cache.  Returns [n_nodes, n_heads, d_value].
+    torch::Tensor forward_draft(torch::Tensor q, torch::Tensor k, torch::Tensor v, DraftBatch& draft);
+    // Continue the rows named in `rows` by the given tokens and their keys and values (k, v: all rows' tokens, laid end to end), as accepting
+    // drafted tokens does.  A row may get none.
+    void extend_kv(const std::vector<int>& rows, const std::vector<std::vector<int>>& tokens, torch::Tensor k, torch::Tensor v);
     // ---- latent caches ----
     // Projections [n_tokens, query latent | key/value latent | shared key part] to the pool; returns the normalised query
     // latents [n_tokens, q_rank].  append_tokens as in store_qkv.
@@ -183,6 +192,17 @@ class Attention {
         std::vector<int> starts, lens;  // first position and tokens of every entry
     };
     std::shared_ptr<Tables> tables_;
+    // The work list of the drafted trees at hand, shared in the same way.
+    struct DraftWork {
+        int64_t serial = -1;
+        std::vector<ca_chunk_info> infos;
+        Uploaded device;
+        ca_draft_plan_info info{};
+    };
+    std::shared_ptr<std::shared_ptr<DraftWork>> shared_draft_;
+    std::shared_ptr<DraftWork> draft_;
+    int64_t draft_version_ = -1, draft_appended_ = -1;  // of the tree, when draft_ was found to be of it
+    std::vector<torch::Tensor> captured_;               // buffers that captured steps read
     const std::pair<torch::Tensor, int>& blocks_of(int block_rows);
     const WindowTables& window_tables();
     void need_latent(const char* what) const;

@@ -17,6 +17,7 @@ using ca_host::PrefixTree;
 namespace ca_host {
 void init_ops(py::module& m);
 void init_block_ops(py::module& m, py::module& ops);
+void init_draft(py::module& m, py::module& ops);
 }
 
 namespace {
@@ -137,6 +138,8 @@ PYBIND11_MODULE(chunk_attn_c, m) {
            py::arg("value_freq") = py::none(), py::arg("append_tokens") = py::none())
       .def("forward_rows", &Attention::forward_rows, py::arg("q"), py::arg("positions"), py::arg("value_freq") = py::none(),
            py::arg("row_entry") = py::none())
+      .def("forward_draft", &Attention::forward_draft, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("draft"))
+      .def("extend_kv", &Attention::extend_kv, py::arg("rows"), py::arg("tokens"), py::arg("k"), py::arg("v"))
       .def("forward", &Attention::forward, py::arg("q"), py::arg("partition") = 0)
       .def("add_seq", &Attention::add_seq, py::arg("tokens"), py::arg("k"), py::arg("v"))
       .def("add_seq_async", &Attention::add_seq_async, py::arg("tokens"), py::arg("k"), py::arg("v"))
@@ -179,6 +182,7 @@ PYBIND11_MODULE(chunk_attn_c, m) {
     py::module ops = m.def_submodule("ops");
     ca_host::init_ops(ops);
     ca_host::init_block_ops(m, ops);
+    ca_host::init_draft(m, ops);
 
     py::class_<PrefixTree>(m, "PrefixTree", py::module_local())
       .def(py::init([](int chunk_size, int64_t max_chunks, bool share_prefix) {

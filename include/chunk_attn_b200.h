@@ -637,6 +637,91 @@ CA_API int ca_plan_build_for_context(const ca_context* ctx, ca_plan** out, const
 CA_API int ca_refresh_from_plan(ca_context* ctx, const ca_plan* plan, ca_stream stream);
 CA_API void ca_plan_destroy(ca_plan* plan);
 
+/* ---- drafted tokens ---------------------------------------------------------------------------------------------
+ * Attention of trees of drafted tokens over the cache: every row of the cache brings a tree of nodes, node i sees the cached
+ * tokens of its row, its ancestors in the tree and itself.  Drafted keys and values are operands; nothing is written to
+ * the pool.  Fixed-geometry contexts and contexts with a head shape (not latent), every type and geometry that they serve.
+ *
+ * The work list is made on the host from the chunk list and the first node of every row's tree (first[0 .. n_rows]), once per step for
+ * all layers; ca_draft_plan_data gives it as one array for the caller to bring to the device.  block_rows: query rows of an item
+ * (ca_draft_plan_for_context: as the context's kernels want it). */
+#define CA_DRAFT_MAX_NODES 256 /* nodes of a tree */
+typedef struct ca_draft_plan ca_draft_plan;
+typedef struct ca_draft_plan_info {
+    int32_t n_items, n_merge, n_slots, n_nodes;
+    int32_t block_rows;    /* query rows of an item at most                                               */
+    int32_t longest;       /* tokens of the longest item                                                  */
+    int64_t n_data;        /* int32 entries of the array: items at 0, the other parts at ...              */
+    int64_t at_tiles, at_nodes, at_off, at_slots;
+} ca_draft_plan_info;
+CA_API int ca_draft_plan_build(ca_draft_plan** out, const ca_chunk_info* infos, int n_infos, const int32_t* first, int n_rows,
+                               int chunk_size, int tpp_threshold, int64_t max_chunks, int kv_heads, int group, int block_rows, int ctas);
+CA_API int ca_draft_plan_for_context(const ca_context* ctx, ca_draft_plan** out, const ca_chunk_info* infos, int n_infos,
+                                     const int32_t* first, int n_rows);
+CA_API int ca_draft_plan_data(const ca_draft_plan* plan, const int32_t** data, ca_draft_plan_info* info);
+CA_API void ca_draft_plan_destroy(ca_draft_plan* plan);
+
+typedef struct ca_draft_args {
+    const void* q;              /* [n_nodes, n_heads, d_key], element strides q_node, q_head; elements of a head contiguous */
+    const void* k;              /* [n_nodes, n_kv_heads, d_key]                       */
+    const void* v;              /* [n_nodes, n_kv_heads, d_value]                     */
+    int64_t q_node, q_head, k_node, k_head, v_node, v_head;
+    void* out;                  /* [n_nodes, n_heads, d_value] contiguous, 16-byte aligned */
+    const uint32_t* seen;       /* device [n_nodes][words]: bit j: node j of the same tree is the node itself or above it */
+    int32_t words;              /* even                                               */
+    const int32_t* work;        /* device: the plan's array                           */
+    const ca_draft_plan_info* info;
+    float* partials;            /* device scratch of ca_draft_partial_floats floats   */
+} ca_draft_args;
+CA_API int64_t ca_draft_partial_floats(const ca_context* ctx, const ca_draft_plan_info* info);
+CA_API int ca_draft_attention(ca_context* ctx, const ca_draft_args* args, ca_stream stream);
+
+/* Which drafted tokens are accepted.  tokens: the drafted token of every node; choice: the token that the model takes after every
+ * node.  A node is good when its token is its parent's choice, or, with log_probs (of the node's token after its parent) and
+ * entropy (of the distribution after every node), when log_probs >= min(log(epsilon), log(delta) - entropy of the parent).  Of every tree
+ * the deepest node whose line of ancestors is good is taken (of equal ones the first), the first node of a tree always being so:
+ * path [n_rows, width] gets the line's nodes, numbered within the tree, then -1; count its length; next the choice after its end.
+ * A tree without nodes: count 0, next -1.  Device pointers; first [n_rows + 1], parent and depth [n_nodes], seen as above; every
+ * tree has one node without a parent, its first; width >= the deepest node's depth + 1. */
+typedef struct ca_accept_args {
+    const int32_t* first;
+    const int32_t* parent;
+    const int32_t* depth;
+    const uint32_t* seen;
+    int32_t words, n_rows, width;
+    const int32_t* tokens;
+    const int32_t* choice;
+    const float* log_probs;     /* NULL: the choice only */
+    const float* entropy;
+    double epsilon, delta;
+    int32_t* path;
+    int32_t* count;
+    int32_t* next;
+} ca_accept_args;
+CA_API int ca_accept_draft(const ca_accept_args* args, ca_stream stream);
+
+/* Log probabilities from logits [n_rows, vocab] (any type, rows row_stride elements apart): with lse = log sum exp of a row,
+ * log_probs[i] = logits[rows[i]][tokens[i]] - lse (rows NULL: i; token -1: 0; other ids or rows out of range: NaN),
+ * entropy[r] = lse - sum p x, and the top best tokens of a row by value, of equal ones those with the lowest ids:
+ * top_ids, top_log_probs [n_rows, top].  Excluded tokens (-infinity) have probability 0.  A row that holds a NaN, +infinity or nothing
+ * but -infinity has no distribution: its numbers are NaN (top_ids counts NaN as -infinity).  scratch: ca_log_probs_scratch bytes. */
+#define CA_MAX_TOP 32
+typedef struct ca_log_probs_args {
+    const void* logits;
+    int64_t row_stride;
+    int32_t n_rows, vocab, dtype;
+    const int32_t* tokens;
+    const int32_t* rows;
+    int32_t n_tokens, top;
+    float* log_probs;           /* [n_tokens] */
+    float* entropy;             /* [n_rows]   */
+    float* top_log_probs;
+    int32_t* top_ids;
+    void* scratch;
+} ca_log_probs_args;
+CA_API int64_t ca_log_probs_scratch(int n_rows, int vocab, int dtype, int top);
+CA_API int ca_token_log_probs(const ca_log_probs_args* args, ca_stream stream);
+
 #ifdef __cplusplus
 }
 #endif
