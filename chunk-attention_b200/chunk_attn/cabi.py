@@ -21,6 +21,7 @@ CA_OPT_SPAN_TENSOR = 11
 CA_OPT_DIRECT = 12
 CA_OPT_FINISH_IN_WIDE = 13
 CA_OPT_LATENT_ROWS = 14
+CA_OPT_DRAFT_TENSOR = 15
 STATUS_FULL_WAIT_TIMEOUT, STATUS_EMPTY_WAIT_TIMEOUT, STATUS_DRAIN_TIMEOUT, STATUS_BAD_WORK_LIST, STATUS_BAD_POSITION = 1, 2, 3, 4, 5
 PLAN_ITEMS = 0
 (PLAN_MERGE_OFF, PLAN_MERGE_SLOTS, PLAN_PATH_OFF, PLAN_PATH_CHUNKS, PLAN_PATH_TOKENS, PLAN_TAIL_CHUNK,

@@ -127,6 +127,7 @@ struct ca_context {
     int trace_ctas = 0;                   // CTAs of the last traced launch
     int trace_cycles = 0;                 // CA_OPT_TRACE = 2: the tcgen05 kernel accounts for cycles per role instead
     int opt_direct = 1;                   // CA_OPT_DIRECT
+    int opt_draft_tensor = 1;             // CA_OPT_DRAFT_TENSOR
     int opt_finish_in_wide = 1;           // CA_OPT_FINISH_IN_WIDE
     int opt_latent_rows = 1;              // CA_OPT_LATENT_ROWS
     int opt_finish_in_tails = 1;          // CA_OPT_FINISH_IN_TAILS: the short-tails kernel finishes the rows when it can
@@ -360,6 +361,10 @@ int ca_context_set_option(ca_context* c, int option, int64_t value) {
     } else if (option == CA_OPT_LATENT_ROWS) {
         if (value < 0 || value > 2) return fail(CA_ERR_INVALID, "CA_OPT_LATENT_ROWS takes 0, 1 or 2");
         c->opt_latent_rows = (int)value;
+        return CA_OK;
+    } else if (option == CA_OPT_DRAFT_TENSOR) {
+        if (value < 0 || value > 1) return fail(CA_ERR_INVALID, "CA_OPT_DRAFT_TENSOR takes 0 or 1");
+        c->opt_draft_tensor = (int)value;
         return CA_OK;
     } else if (option == CA_OPT_SPAN_TENSOR) {
         if (value < 0 || value > 2) return fail(CA_ERR_INVALID, "CA_OPT_SPAN_TENSOR takes 0, 1 or 2");
@@ -1731,6 +1736,11 @@ int ca_draft_plan_build(ca_draft_plan** out, const ca_chunk_info* infos, int n_i
     return make_draft_plan(out, infos, n_infos, first, n_rows, shape);
 }
 
+static float draft_scale(const ca_context* c) { return c->shaped ? c->shape.scale : 1.f / std::sqrt((float)c->geo.d_head); }
+static bool draft_on_tensor_cores(const ca_context* c) {
+    return c->opt_draft_tensor && ca::draft_tc_serves(c->geo, c->shaped ? c->shape.d_key : c->geo.d_head, c->shaped ? c->shape.d_value : c->geo.d_head, c->group, draft_scale(c));
+}
+
 int ca_draft_plan_for_context(const ca_context* c, ca_draft_plan** out, const ca_chunk_info* infos, int n_infos, const int32_t* first, int n_rows) {
     if (!c || !out || !first || n_rows < 0) return fail(CA_ERR_INVALID, "null or negative argument");
     if (c->shape.latent) return fail(CA_ERR_INVALID, "drafted tokens: a latent cache is not served");
@@ -1750,9 +1760,14 @@ int ca_draft_plan_for_context(const ca_context* c, ca_draft_plan** out, const ca
     for (int i = 0; i < n_infos; i++)
         if (infos && infos[i].n_tokens > 0 && infos[i].seq_begin >= 0 && infos[i].seq_end <= n_rows && infos[i].seq_end - infos[i].seq_begin > c->tpp_threshold)
             widest = std::max(widest, first[infos[i].seq_end] - first[infos[i].seq_begin]);
-    shape.block_rows = ca::draft_generic_rows(std::min(widest, 64) * c->group);
-    shape.ctas = 4 * ca::B200_SMS;
-    if (c->group > shape.block_rows) return fail(CA_ERR_INVALID, "drafted tokens: more than 64 query heads to a key/value head");
+    if (draft_on_tensor_cores(c)) {
+        shape.block_rows = ca::DRAFT_TC_ROWS;
+        shape.ctas = 2 * ca::B200_SMS;
+    } else {
+        shape.block_rows = ca::draft_generic_rows(std::min(widest, 64) * c->group);
+        shape.ctas = 4 * ca::B200_SMS;
+    }
+    if (c->group > 64) return fail(CA_ERR_INVALID, "drafted tokens: more than 64 query heads to a key/value head");
     return make_draft_plan(out, infos, n_infos, first, n_rows, shape);
 }
 
@@ -1814,7 +1829,7 @@ int ca_draft_attention(ca_context* c, const ca_draft_args* a, ca_stream stream_)
     p.v_node = a->v_node;
     p.v_head = a->v_head;
     p.out = a->out;
-    p.scale_log2 = (c->shaped ? c->shape.scale : 1.f / std::sqrt((float)c->geo.d_head)) * 1.4426950408889634f;
+    p.scale_log2 = draft_scale(c) * 1.4426950408889634f;
     p.sink = c->shaped ? c->shape.sink : 0;
     p.seen = a->seen;
     p.words = a->words;
@@ -1829,11 +1844,23 @@ int ca_draft_attention(ca_context* c, const ca_draft_args* a, ca_stream stream_)
     p.merge_off = a->work + a->info->at_off;
     p.merge_slots = a->work + a->info->at_slots;
     p.n_merge = a->info->n_merge;
+    p.n_list = (int)((a->info->at_nodes - a->info->at_tiles) / 2);
+    p.n_slots = a->info->n_slots;
     p.max_chunks = (int)c->max_chunks;
     p.status = c->status;
     p.wait_limit = c->opt_wait_limit;
     p.dependent = c->opt_pdl;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (a->info->block_rows == ca::DRAFT_TC_ROWS) {
+        if (!draft_on_tensor_cores(c)) return fail(CA_ERR_STATE, "drafted tokens: the work list was made for other kernels");
+        // tensor copies: addresses and strides of whole 16-byte units
+        auto whole = [](const void* t, int64_t node, int64_t head) { return reinterpret_cast<uintptr_t>(t) % 16 == 0 && node % 8 == 0 && head % 8 == 0 && node > 0 && head > 0; };
+        if (!whole(a->q, a->q_node, a->q_head) || !whole(a->k, a->k_node, a->k_head) || !whole(a->v, a->v_node, a->v_head))
+            return fail(CA_ERR_INVALID, "drafted tokens: operands of 16-bit caches must be 16-byte aligned, with strides of whole 16 bytes");
+        CA_CUDA(ca::launch_draft_tc(p, c->dtype, stream));
+        CA_CUDA(ca::launch_draft_merge(p, c->dtype, stream));
+        return CA_OK;
+    }
     CA_CUDA(ca::launch_draft_generic(p, a->info->block_rows, c->dtype, stream));
     CA_CUDA(ca::launch_draft_merge(p, c->dtype, stream));
     return CA_OK;

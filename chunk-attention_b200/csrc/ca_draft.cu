@@ -43,7 +43,12 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
     const int G = p.geo.n_heads, group = p.group, H = G * group, C = p.geo.chunk_size;
     const int kvh = blockIdx.x % G;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const DraftItem it = p.items[blockIdx.x / G];
+    const int4 ia = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G)), ib = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 1);
+    const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w};
+    if (!draft_item_ok(p, ia, ib, G_WARPS * RW)) {
+        if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
+        return;
+    }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int n_rows = it.n_nodes * group;
 

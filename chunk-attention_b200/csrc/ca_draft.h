@@ -74,17 +74,26 @@ struct DraftParams {
     int part_width;
     const int32_t *merge_nodes, *merge_off, *merge_slots;
     int n_merge;
+    int n_list, n_slots;       // entries of tiles, partial slots
     int max_chunks;
     int* status;
     long long wait_limit;
     int dependent;             // CA_OPT_DEPENDENT_LAUNCH
 };
+// nothing in a work list is trusted
+__device__ __forceinline__ bool draft_item_ok(const DraftParams& p, int4 a, int4 b, int block_rows) {
+    return a.x >= 0 && a.y > 0 && a.x + a.y <= p.n_nodes && a.y * p.group <= block_rows && a.z >= 0 && a.w >= 0 && a.z + a.w <= p.n_list &&
+           b.x + a.y <= p.n_slots + (b.x < 0 ? a.y : 0) && b.y >= 0 && b.z >= 0 && b.y + b.z <= p.n_nodes && b.z <= 32 * p.words && a.w + b.z > 0;
+}
 #endif
 // query rows of an item that the any-geometry kernel takes, for units of so many
 inline int draft_generic_rows(int unit_rows) { return unit_rows <= 16 ? 16 : (unit_rows <= 32 ? 32 : 64); }
 
 #if defined(__CUDACC__)
 cudaError_t launch_draft_generic(const DraftParams& p, int block_rows, int dtype, cudaStream_t stream);
+bool draft_tc_serves(const Geometry& g, int d_key, int d_value, int group, float scale);
+cudaError_t launch_draft_tc(const DraftParams& p, int dtype, cudaStream_t stream);
+constexpr int DRAFT_TC_ROWS = 128;  // query rows of an item
 cudaError_t launch_draft_merge(const DraftParams& p, int dtype, cudaStream_t stream);
 
 struct AcceptParams {

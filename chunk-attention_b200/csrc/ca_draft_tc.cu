@@ -1,0 +1,582 @@
+// Attention of drafted trees on the Blackwell tensor path: tcgen05.mma (fp16 or bf16) with accumulators in tensor memory.  For caches of
+// 64-token chunks and head sizes of 64 or 128 elements, whose pool tiles are the tensor cores' own 128-byte-swizzled operand layout.
+//
+// A piece of work is (item, key/value head): up to 128 query rows (the query heads of a group for consecutive nodes; row r is head r % group of
+// node r / group) against the item's chunks and, in the last piece of a row's private part, the drafted keys and values.
+//   S = Q K^T      M = 128 rows, N = 64 tokens; D in TMEM, two buffers, so that S of tile j + 1 is computed under the softmax of tile j
+//   softmax        one thread per row (= TMEM lane), fp32, log2 units; O is rescaled only when a row's maximum has grown by more than 8.
+//                  The weights go back over S as hi + lo parts, whose sum has 16 bits of the fp32 weight (bf16; fp16: 22), so that what
+//                  is left of rounding is that of the result
+//   O += P V       A = P from TMEM, B = the V tile (MN-major panels)
+// Pool tiles are bulk-copied verbatim; queries and drafted keys and values come by TMA tensor copies, which lay them out alike.  A drafted
+// tile is masked by the bits of a row's line.  Rows leave as finished 16-bit rows where the item serves its nodes whole, else as
+// fp32 partial results.
+// Warp roles: 0-3 softmax and epilogue, 4 TMA producer over a ring of four tile slots, 5 TMEM and the MMA issue, 6 the next piece
+// of work (a CTA takes over pieces that have not been launched yet: cluster launch control).  Two CTAs share an SM.
+//
+// A row of which an element comes out as not finite is computed once more on CUDA cores: a value that is infinite may be one that the row does
+// not see (0 * infinity), and hi + lo parts of a weight times infinity are not its product.
+//
+// Every wait is bounded: on expiry a status code is recorded, every role falls through to the common exit, and the TMEM columns are
+// freed there.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "ca_draft.h"
+#include "ca_kernels.h"
+#include "ca_launch.cuh"
+#include "ca_ptx.cuh"
+#include "ca_softmax.cuh"
+#include "ca_tensor_map.h"
+#include "ca_types.cuh"
+
+namespace ca {
+namespace {
+using namespace ptx;
+
+constexpr int A_ROWS = 128, A_TOK = 64, A_SLOTS = 4, A_THREADS = 256;
+constexpr int A_SOFTMAX_REGS = 200, A_OTHER_REGS = 56;  // per thread; the block is launched with 2 x 128 (checked at the launch)
+constexpr int A_TMEM_COLS = 256, A_COL_S = 128;
+constexpr int A_NUM_BARS = 2 * A_SLOTS + 13;
+constexpr float A_NEG_BIG = -1.0e30f, A_RESCALE_STEP = 8.f;
+
+template <typename T> __host__ __device__ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
+    return umma_idesc_f16(A_ROWS, n, false, b_mn_major) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
+}
+__device__ __forceinline__ void report(int* status, int code) { atomicCAS(status, STATUS_OK, code); }
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        return pack_half2(lo, hi);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+// 32 weights as pairs, and what their rounding left out
+template <typename T> __device__ __forceinline__ void split_tile(const uint32_t (&s)[32], uint32_t* hi, uint32_t* lo) {
+    if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float a = __uint_as_float(s[2 * i]), b = __uint_as_float(s[2 * i + 1]);
+            hi[i] = pack_half2(a, b);
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+            lo[i] = pack_half2(a - h.x, b - h.y);
+        }
+    } else {
+        split_weights(s, hi, lo);
+    }
+}
+
+// A piece of work as the roles read it; n_tiles = 0: there is none left
+struct alignas(16) Work {
+    int node0, n_rows, n_tiles, n_context;  // tiles in all, and from the pool
+    int list, tree, n_drafted, slot;
+    int n_nodes, kvh, pad[2];
+};
+
+template <int DK, int DV> struct Sizes {
+    static constexpr int Q_BYTES = A_ROWS * DK * 2, Q_PANEL = A_ROWS * 128;
+    static constexpr int K_BYTES = A_TOK * DK * 2, V_BYTES = A_TOK * DV * 2;
+    static constexpr int SLOT = K_BYTES > V_BYTES ? K_BYTES : V_BYTES;
+    static constexpr int OUT_PITCH = 64 + 16;  // 64 bytes of a row at a time
+    static constexpr int OUT = Q_BYTES + A_SLOTS * SLOT;
+    static constexpr int WORK = OUT + A_ROWS * OUT_PITCH, CLC = WORK + 2 * (int)sizeof(Work), BARS = CLC + 16;
+    static constexpr int SMEM = BARS + A_NUM_BARS * 8 + 8;
+};
+
+// One row of a piece once more, by a warp: lane e has the elements e, e + 32, ...
+template <typename T>
+__device__ __noinline__ void row_again(const DraftParams& p, const Work& w, int r, int lane) {
+    const int G = p.geo.n_heads, group = p.group, H = G * group, dk = p.d_key, dv = p.d_value;
+    const int node = w.node0 + r / group, head = w.kvh * group + r % group;
+    const T* q = static_cast<const T*>(p.q) + (int64_t)node * p.q_node + (int64_t)head * p.q_head;
+    float qe[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = A_NEG_BIG, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) qe[i] = lane + 32 * i < dk ? to_f32(q[lane + 32 * i]) : 0.f;
+    const Geometry vs = tile_side(p.geo, 1);
+    auto take = [&](auto key, auto value) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (lane + 32 * i < dk) s = fmaf(qe[i], key(lane + 32 * i), s);
+        s = warp_sum(s) * p.scale_log2;
+        const float mn = fmaxf(m, s), alpha = exp2f(m - mn), x = exp2f(s - mn);
+        m = mn;
+        l = l * alpha + x;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (lane + 32 * i < dv) o[i] = o[i] * alpha + x * value(lane + 32 * i);
+    };
+    for (int j = 0; j < w.n_context; j++) {
+        const int chunk = p.tiles[2 * (w.list + j)], n = min(p.tiles[2 * (w.list + j) + 1], A_TOK);
+        if (chunk < 0 || chunk >= p.max_chunks) continue;
+        const T* kt = static_cast<const T*>(p.pool) + tile_base_elems(p.geo, chunk, w.kvh, 0);
+        const T* vt = kt + p.geo.tile_elems;
+        for (int t = 0; t < n; t++)
+            take([&](int e) { return to_f32(kt[tile_elem_offset(p.geo, t, e)]); }, [&](int e) { return to_f32(vt[tile_elem_offset(vs, t, e)]); });
+    }
+    for (int t = 0; t < w.n_drafted; t++) {
+        if (!((p.seen[(int64_t)node * p.words + t / 32] >> (t & 31)) & 1)) continue;
+        const T* k = static_cast<const T*>(p.k) + (int64_t)(w.tree + t) * p.k_node + (int64_t)w.kvh * p.k_head;
+        const T* v = static_cast<const T*>(p.v) + (int64_t)(w.tree + t) * p.v_node + (int64_t)w.kvh * p.v_head;
+        take([&](int e) { return to_f32(k[e]); }, [&](int e) { return to_f32(v[e]); });
+    }
+    if (w.slot >= 0) {
+        const int64_t at = (int64_t)(w.slot + node - w.node0) * H + head;
+        if (lane == 0) p.part_ml[at] = make_float2(m, l);
+        for (int i = 0; i < 4; i++)
+            if (lane + 32 * i < dv) p.part_o[at * p.part_width + lane + 32 * i] = o[i];
+    } else {
+        const float M = p.sink ? fmaxf(m, 0.f) : m, x = exp2f(m - M), total = l * x + (p.sink ? exp2f(-M) : 0.f);
+        for (int i = 0; i < 4; i++)
+            if (lane + 32 * i < dv) static_cast<T*>(p.out)[((int64_t)node * H + head) * dv + lane + 32 * i] = from_f32<T>(total == 0.f ? 0.f : o[i] * x / total);
+    }
+}
+
+template <typename T, int DK, int DV>
+__global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_constant__ DraftParams p, const __grid_constant__ CUtensorMap q_map,
+                                                                  const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    using Z = Sizes<DK, DV>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t sbase = smem_u32(smem);
+    const uint32_t ring = sbase + Z::Q_BYTES;
+    const uint32_t full_bar = sbase + Z::BARS;
+    const uint32_t empty_bar = full_bar + 8 * A_SLOTS;
+    const uint32_t s_full = empty_bar + 8 * A_SLOTS;  // [2]
+    const uint32_t p_full = s_full + 16;              // [2]
+    const uint32_t work_full = p_full + 16;           // [2]
+    const uint32_t work_empty = work_full + 16;       // [2]
+    const uint32_t o_done = work_empty + 16;
+    const uint32_t o_free = o_done + 8;
+    const uint32_t q_full = o_free + 8;
+    const uint32_t q_empty = q_full + 8;
+    const uint32_t clc_bar = q_empty + 8;
+    Work* const work = reinterpret_cast<Work*>(smem + Z::WORK);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Z::BARS + A_NUM_BARS * 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = p.geo.n_heads, group = p.group, H = G * group;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < A_SLOTS; i++) {
+            mbar_init(full_bar + 8 * i, 1);
+            mbar_init(empty_bar + 8 * i, 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(s_full + 8 * b, 1);
+            mbar_init(p_full + 8 * b, 4 * 32);
+            mbar_init(work_full + 8 * b, 1);
+            mbar_init(work_empty + 8 * b, 4 * 32 + 2);
+        }
+        mbar_init(o_done, 1);
+        mbar_init(o_free, 4 * 32);
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        mbar_init(clc_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 5) {  // the warp that allocates is the warp that frees
+        tmem_alloc(smem_u32(tmem_slot), A_TMEM_COLS);
+        tmem_relinquish_alloc_permit();
+    }
+    tc_fence_before_thread_sync();
+    __syncthreads();
+    tc_fence_after_thread_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    // with tensor memory in hand: a kernel behind this one may allocate, too
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // a wait of a single thread: false, with the code recorded, when the limit ran out
+    auto wait = [&](uint32_t bar, int parity, int code) {
+        if (mbar_wait_bounded(bar, parity, p.wait_limit)) return true;
+        report(p.status, code);
+        return false;
+    };
+
+    if (warp >= 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(A_OTHER_REGS));
+        if (warp == 6 && lane == 0) {
+            // ---- the next piece of work, asked for when the piece before the present one is finished
+            int item = blockIdx.x;
+            for (int n = 0;; n++) {
+                if (n > 0) {
+                    if (!wait(work_empty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, STATUS_EMPTY_WAIT_TIMEOUT)) break;
+                    mbar_arrive_expect_tx(clc_bar, 16);
+                    clc_try_cancel(sbase + Z::CLC, clc_bar);
+                    if (!wait(clc_bar, (n - 1) & 1, STATUS_FULL_WAIT_TIMEOUT)) {
+                        wait(clc_bar, (n - 1) & 1, STATUS_DRAIN_TIMEOUT);  // the answer is still on its way into this CTA's memory
+                        break;
+                    }
+                    item = clc_block(sbase + Z::CLC);
+                    fence_proxy_async();  // read before the next answer is written
+                }
+                Work w{};
+                if (item >= 0) {
+                    const int4* it = reinterpret_cast<const int4*>(p.items + item / G);
+                    const int4 a = __ldg(it), b = __ldg(it + 1);
+                    w.node0 = a.x;
+                    w.n_nodes = a.y;
+                    w.n_rows = a.y * group;
+                    w.list = a.z;
+                    w.n_context = a.w;
+                    w.slot = b.x;
+                    w.tree = b.y;
+                    w.n_drafted = b.z;
+                    w.n_tiles = a.w + (b.z + A_TOK - 1) / A_TOK;
+                    w.kvh = item % G;
+                    if (!draft_item_ok(p, a, b, A_ROWS)) {  // this CTA ends; pieces that have not been launched are others'
+                        report(p.status, STATUS_BAD_WORK_LIST);
+                        w.n_tiles = 0;
+                        item = -1;
+                    }
+                }
+                work[n & 1] = w;
+                mbar_arrive(work_full + 8 * (n & 1));
+                if (item < 0) break;
+            }
+        } else if (warp == 4 && lane == 0) {
+            // ---- producer: slot i & 3 takes K of tile i / 2 (even i) or its V (odd i), i counted over all pieces
+            int issued = 0, q_issued = 0, n = 0;
+            for (bool live = true; live; n++) {
+                if (!wait(work_full + 8 * (n & 1), (n >> 1) & 1, STATUS_FULL_WAIT_TIMEOUT)) break;
+                const Work w = work[n & 1];
+                mbar_arrive(work_empty + 8 * (n & 1));
+                if (w.n_tiles == 0) break;
+                const int2* tiles = reinterpret_cast<const int2*>(p.tiles) + w.list;
+                int2 tile = w.n_context > 0 ? __ldg(tiles) : make_int2(0, 0);
+                for (int j = 0; j < w.n_tiles && live; j++) {
+                    const int2 next = j + 1 < w.n_context ? __ldg(tiles + j + 1) : make_int2(0, 0);  // on its way while slots are waited for
+                    if (j < w.n_context && (tile.x < 0 || tile.x >= p.max_chunks || tile.y <= 0 || tile.y > A_TOK)) {
+                        report(p.status, STATUS_BAD_WORK_LIST);  // keep the pipeline moving on a chunk that exists
+                        tile = make_int2(0, A_TOK);
+                    }
+                    const uint8_t* src = static_cast<const uint8_t*>(p.pool) + ((size_t)tile.x * G + w.kvh) * (size_t)(Z::K_BYTES + Z::V_BYTES);
+                    for (int side = 0; side < 2; side++) {
+                        const int slot = issued & (A_SLOTS - 1);
+                        if (!wait(empty_bar + 8 * slot, ((issued / A_SLOTS) & 1) ^ 1, STATUS_EMPTY_WAIT_TIMEOUT)) {
+                            live = false;
+                            break;
+                        }
+                        const uint32_t dst = ring + slot * Z::SLOT, bar = full_bar + 8 * slot;
+                        const int panels = side ? DV / 64 : DK / 64;
+                        if (j < w.n_context) {
+                            const uint8_t* from = src + side * Z::K_BYTES;
+                            mbar_arrive_expect_tx(bar, panels * tile.y * 128);
+                            if (tile.y == A_TOK) {
+                                bulk_copy_g2s(dst, from, panels * A_TOK * 128, bar);
+                            } else {
+                                for (int pn = 0; pn < panels; pn++) bulk_copy_g2s(dst + pn * (A_TOK * 128), from + pn * (A_TOK * 128), tile.y * 128, bar);
+                            }
+                        } else {
+                            // lines past the drafted nodes are other trees' or zeros
+                            mbar_arrive_expect_tx(bar, panels * A_TOK * 128);
+                            for (int pn = 0; pn < panels; pn++)
+                                tma_load_3d(dst + pn * (A_TOK * 128), side ? &v_map : &k_map, 64 * pn, w.kvh, w.tree + (j - w.n_context) * A_TOK, bar);
+                        }
+                        issued++;
+                        if (j == 0 && side == 0) {
+                            // the queries follow the first K tile.  Rows past the block are other nodes' or zeros: nobody reads theirs
+                            if (!wait(q_empty, (n & 1) ^ 1, STATUS_EMPTY_WAIT_TIMEOUT)) {
+                                live = false;
+                                break;
+                            }
+                            mbar_arrive_expect_tx(q_full, (DK / 64) * (A_ROWS / group) * group * 128);
+#pragma unroll
+                            for (int pn = 0; pn < DK / 64; pn++) tma_load_3d(sbase + pn * Z::Q_PANEL, &q_map, 64 * pn, w.kvh * group, w.node0, q_full);
+                            q_issued++;
+                        }
+                    }
+                    tile = next;
+                }
+            }
+            for (int f = issued > A_SLOTS ? issued - A_SLOTS : 0; f < issued; f++)
+                if (!wait(full_bar + 8 * (f & (A_SLOTS - 1)), (f / A_SLOTS) & 1, STATUS_DRAIN_TIMEOUT)) break;
+            if (q_issued > 0) wait(q_full, (q_issued - 1) & 1, STATUS_DRAIN_TIMEOUT);  // pieces begun may be one more
+        } else if (warp == 5 && elect_one()) {
+            // ---- MMA issuer: one thread; t counts tiles over all pieces
+            constexpr uint32_t DESC_HI = umma_desc_sw128_hi(1024);
+            constexpr uint32_t IDESC_QK = idesc_of<T>(A_TOK, false), IDESC_PV = idesc_of<T>(DV, true);
+            const uint32_t q_lo = umma_desc_sw128_lo(sbase, 16);
+            auto issue_qk = [&](int t) {
+                const int i = 2 * t, slot = i & (A_SLOTS - 1);
+                if (!wait(full_bar + 8 * slot, (i / A_SLOTS) & 1, STATUS_FULL_WAIT_TIMEOUT)) return false;
+                tc_fence_after_thread_sync();
+                const uint32_t d = tmem_base + A_COL_S + (t & 1) * A_TOK;
+                const uint32_t b_lo = umma_desc_sw128_lo(ring + slot * Z::SLOT, 16);
+#pragma unroll
+                for (int ks = 0; ks < DK / 16; ks++) {
+                    const uint64_t a = umma_desc_pack(q_lo + (((ks >> 2) * Z::Q_PANEL + (ks & 3) * 32) >> 4), DESC_HI);
+                    const uint64_t b = umma_desc_pack(b_lo + (((ks >> 2) * (A_TOK * 128) + (ks & 3) * 32) >> 4), DESC_HI);
+                    umma_ss_f16(d, a, b, IDESC_QK, ks > 0 ? 1u : 0u);
+                }
+                umma_commit(s_full + 8 * (t & 1));
+                umma_commit(empty_bar + 8 * slot);
+                return true;
+            };
+            int t = 0;
+            bool live = true;
+            for (int n = 0; live; n++) {
+                if (!wait(work_full + 8 * (n & 1), (n >> 1) & 1, STATUS_FULL_WAIT_TIMEOUT)) break;
+                const int n_tiles = work[n & 1].n_tiles;
+                mbar_arrive(work_empty + 8 * (n & 1));
+                if (n_tiles == 0) break;
+                live = wait(q_full, n & 1, STATUS_FULL_WAIT_TIMEOUT) && issue_qk(t);
+                if (live && n_tiles == 1) umma_commit(q_empty);
+                for (int j = 0; j < n_tiles && live; j++, t++) {
+                    if (j + 1 < n_tiles) {
+                        if (!(live = issue_qk(t + 1))) break;
+                        if (j + 2 == n_tiles) umma_commit(q_empty);
+                    }
+                    const int i = 2 * t + 1, slot = i & (A_SLOTS - 1);
+                    live = wait(p_full + 8 * (t & 1), (t >> 1) & 1, STATUS_FULL_WAIT_TIMEOUT) &&
+                           wait(full_bar + 8 * slot, (i / A_SLOTS) & 1, STATUS_FULL_WAIT_TIMEOUT) &&
+                           (j > 0 || wait(o_free, (n & 1) ^ 1, STATUS_FULL_WAIT_TIMEOUT));  // the piece before has read its O
+                    if (!live) break;
+                    tc_fence_after_thread_sync();
+                    const uint32_t a_tmem = tmem_base + A_COL_S + (t & 1) * A_TOK;  // hi parts, then lo parts, two per column
+                    const uint32_t v_lo = umma_desc_sw128_lo(ring + slot * Z::SLOT, A_TOK * 128);
+#pragma unroll
+                    for (int part = 0; part < 2; part++)
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++) {
+                            const uint64_t b = umma_desc_pack(v_lo + ((kk * 2048) >> 4), DESC_HI);
+                            umma_ts_f16(tmem_base, a_tmem + part * 32 + kk * 8, b, IDESC_PV, (j > 0 || kk > 0 || part > 0) ? 1u : 0u);
+                        }
+                    umma_commit(empty_bar + 8 * slot);
+                    umma_commit(o_done);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(A_SOFTMAX_REGS));
+        // ---- softmax: thread r owns query row r = TMEM lane r
+        const int r = threadIdx.x;
+        // a negative scale: the largest score is then that of the negated product
+        const uint32_t flip = p.scale_log2 < 0.f ? 0x80000000u : 0u;
+        const float scale = fabsf(p.scale_log2);
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(warp * 32) << 16);
+        uint8_t* const stage = smem + Z::OUT + warp * 32 * Z::OUT_PITCH;
+        auto wait_all = [&](uint32_t bar, int parity) {  // by a whole warp
+            const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, p.wait_limit));
+            if (!ok && lane == 0) report(p.status, STATUS_FULL_WAIT_TIMEOUT);
+            return ok;
+        };
+        int t = 0;
+        bool live = true;
+        for (int n = 0; live; n++) {
+            if (!wait_all(work_full + 8 * (n & 1), (n >> 1) & 1)) break;
+            const Work w = work[n & 1];
+            if (w.n_tiles == 0) break;
+            const bool active = r < w.n_rows, busy = warp * 32 < w.n_rows;
+            const int my_node = w.node0 + (active ? r / group : 0);
+            const uint2* line = reinterpret_cast<const uint2*>(p.seen + (int64_t)my_node * p.words);
+            float m_used = A_NEG_BIG, l = 0.f;
+            for (int j = 0; j < w.n_tiles; j++, t++) {
+                const int b = t & 1;
+                const bool drafted = j >= w.n_context;
+                const int filled = drafted ? min(A_TOK, w.n_drafted - (j - w.n_context) * A_TOK) : max(0, min(A_TOK, __ldg(p.tiles + 2 * (w.list + j) + 1)));
+                uint2 see = make_uint2(0u, 0u);
+                if (drafted) see = __ldg(line + (j - w.n_context));
+                if (!(live = wait_all(s_full + 8 * b, (t >> 1) & 1))) break;
+                tc_fence_after_thread_sync();
+                float alpha = 1.f;
+                bool rescale = false;
+                if (busy) {
+                    uint32_t s0[32], s1[32];
+                    tmem_ld32(lane_addr + A_COL_S + b * A_TOK, s0);
+                    tmem_ld32(lane_addr + A_COL_S + b * A_TOK + 32, s1);
+                    tmem_wait_ld();
+                    if (flip) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            s0[i] ^= flip;
+                            s1[i] ^= flip;
+                        }
+                    }
+                    if (drafted || filled < A_TOK) {
+                        if (!drafted) {
+                            see.x = filled >= 32 ? 0xffffffffu : (1u << filled) - 1;
+                            see.y = filled >= 64 ? 0xffffffffu : (filled > 32 ? (1u << (filled - 32)) - 1 : 0u);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            if (!((see.x >> i) & 1)) s0[i] = 0xff800000u;
+                            if (!((see.y >> i) & 1)) s1[i] = 0xff800000u;
+                        }
+                    }
+                    const float mx = fmaxf(tile_max(s0, s1) * scale, A_NEG_BIG);
+                    if (j == 0) {
+                        m_used = mx;
+                    } else if (mx > m_used + A_RESCALE_STEP) {
+                        alpha = fast_exp2(m_used - mx);
+                        m_used = mx;
+                        l *= alpha;
+                        rescale = true;
+                    }
+                    l += tile_weights(s0, s1, scale, m_used);
+                    uint32_t pk[32], lo[32];
+                    split_tile<T>(s0, pk, lo);
+                    split_tile<T>(s1, pk + 16, lo + 16);
+                    tmem_st32(lane_addr + A_COL_S + b * A_TOK, pk);
+                    tmem_st32(lane_addr + A_COL_S + b * A_TOK + 32, lo);
+                }
+                // O += P V of tile t - 1 is complete (every thread follows o_done phase by phase)
+                if (j > 0 && !(live = wait_all(o_done, (t - 1) & 1))) break;
+                if (__any_sync(0xffffffffu, rescale)) {
+                    tc_fence_after_thread_sync();
+#pragma unroll 1
+                    for (int c = 0; c < DV / 32; c++) {
+                        uint32_t o[32];
+                        tmem_ld32(lane_addr + c * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_st32(lane_addr + c * 32, o);
+                    }
+                }
+                if (filled < A_TOK) {
+                    // The rows of V behind the tokens meet weights of zero, so they only have to be finite.  Of a pool tile they are not
+                    // copied (the slot's earlier tile, whose MMA of tile t - 2 is complete, may be another sequence's); of a drafted
+                    // one they are other trees', and are overwritten once the tile is there.
+                    const int vi = 2 * t + 1;
+                    if (drafted && !(live = wait_all(full_bar + 8 * (vi & (A_SLOTS - 1)), (vi / A_SLOTS) & 1))) break;
+                    const uint32_t v_slot = ring + (vi & (A_SLOTS - 1)) * Z::SLOT;
+                    const int grans = (A_TOK - filled) * 8;
+                    for (int i = r; i < (DV / 64) * grans; i += 4 * 32)
+                        sts128_zero(v_slot + (i / grans) * (A_TOK * 128) + filled * 128 + (i % grans) * 16);
+                    fence_proxy_async();
+                }
+                tmem_wait_st();
+                tc_fence_before_thread_sync();
+                mbar_arrive(p_full + 8 * b);
+            }
+            if (!live || !(live = wait_all(o_done, (t - 1) & 1))) break;
+            tc_fence_after_thread_sync();
+            // ---- epilogue: finished rows as 16-bit elements, 32 columns at a time through the warp's own shared memory; partial rows as
+            // fp32, 16 columns at a time.  Sums of 0 x show whether an x is not finite.
+            float scale_out = 1.f, check = 0.f;
+            if (w.slot < 0) {
+                float total = l, M = m_used;
+                if (p.sink) {
+                    M = fmaxf(m_used, 0.f);
+                    total = l * fast_exp2(m_used - M) + fast_exp2(-M);
+                }
+                scale_out = total == 0.f ? 0.f : fast_exp2(m_used - M) / total;
+            } else if (active) {
+                p.part_ml[(int64_t)(w.slot + my_node - w.node0) * H + w.kvh * group + r % group] = make_float2(m_used, l);
+            }
+            const int rows_here = min(32, w.n_rows - warp * 32);
+            char* to[4];  // four lanes to a row
+            const int64_t row_bytes = w.slot < 0 ? DV * 2 : p.part_width * 4;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int row = warp * 32 + 8 * k + (lane >> 2), at = row / group, head = w.kvh * group + row % group;
+                char* base = w.slot < 0 ? static_cast<char*>(p.out) : reinterpret_cast<char*>(p.part_o);
+                to[k] = base + ((int64_t)((w.slot < 0 ? w.node0 : w.slot) + at) * H + head) * row_bytes + 16 * (lane & 3);
+            }
+            // A loop, not unrolled: this code runs once a piece, and straight through it the warps waited for instructions
+#pragma unroll 1
+            for (int c = 0; c < DV / 32; c++) {
+                uint32_t o[32];
+                if (busy) {
+                    tmem_ld32(lane_addr + c * 32, o);
+                    tmem_wait_ld();
+                }
+                if (c == DV / 32 - 1) {  // the accumulator may be overwritten
+                    tc_fence_before_thread_sync();
+                    mbar_arrive(o_free);
+                }
+                if (!busy) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i++) check = fmaf(0.f, __uint_as_float(o[i]), check);
+                if (w.slot < 0) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[i] = pack2<T>(__uint_as_float(o[2 * i]) * scale_out, __uint_as_float(o[2 * i + 1]) * scale_out);
+                }
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    if (half == 1 && w.slot < 0) break;
+                    __syncwarp();  // what was staged before has been read
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        *reinterpret_cast<uint4*>(stage + lane * Z::OUT_PITCH + 16 * i) = make_uint4(o[16 * half + 4 * i], o[16 * half + 4 * i + 1], o[16 * half + 4 * i + 2], o[16 * half + 4 * i + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int rr = 8 * k + (lane >> 2);
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * Z::OUT_PITCH + 16 * (lane & 3));
+                        if (rr < rows_here) *reinterpret_cast<uint4*>(to[k] + (w.slot < 0 ? 64 * c : 128 * c + 64 * half)) = v;
+                    }
+                }
+            }
+            const uint32_t again = __ballot_sync(0xffffffffu, active && !(check + 0.f * l == 0.f));
+            if (again) {
+                __syncwarp();  // the rows above have been stored
+                for (uint32_t rest = again; rest; rest &= rest - 1) row_again<T>(p, w, warp * 32 + __ffs(rest) - 1, lane);
+            }
+            mbar_arrive(work_empty + 8 * (n & 1));
+        }
+    }
+    // ---- common exit: nobody touches TMEM after this barrier, then the allocating warp frees it
+    tc_fence_before_thread_sync();
+    __syncthreads();
+    if (warp == 5) {
+        tc_fence_after_thread_sync();
+        tmem_dealloc(tmem_base, A_TMEM_COLS);
+    }
+}
+
+// [nodes][heads][d] in boxes of one panel (64 elements) of some heads of some nodes
+bool make_map(CUtensorMap* m, bool bf16, const void* base, int d, int64_t heads, int64_t nodes, int64_t head_stride, int64_t node_stride, int box_heads, int box_nodes) {
+    const TensorMapEncode encode = tensor_map_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)nodes}, strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)node_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_nodes}, step[3] = {1, 1, 1};
+    return encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DK, int DV>
+cudaError_t launch(const DraftParams& p, cudaStream_t stream) {
+    auto* k = draft_attn_kernel<T, DK, DV>;
+    constexpr int smem = Sizes<DK, DV>::SMEM;
+    static_assert(2 * (smem + 1024) <= 233472, "two CTAs do not fit in one SM's shared memory");
+    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    const int G = p.geo.n_heads, H = G * p.group;
+    CUtensorMap qm, km, vm;
+    if (!make_map(&qm, bf16, p.q, DK, H, p.n_nodes, p.q_head, p.q_node, p.group, A_ROWS / p.group) ||
+        !make_map(&km, bf16, p.k, DK, G, p.n_nodes, p.k_head, p.k_node, 1, A_TOK) || !make_map(&vm, bf16, p.v, DV, G, p.n_nodes, p.v_head, p.v_node, 1, A_TOK))
+        return cudaErrorInvalidValue;
+    // with fewer registers the warps would wait for them for good; what the compiler gave the kernel does not change
+    static std::atomic<bool> ready;
+    if (!ready) {
+        cudaFuncAttributes have;
+        cudaError_t e = cudaFuncGetAttributes(&have, k);
+        if (e == cudaSuccess && 2 * have.numRegs < A_SOFTMAX_REGS + A_OTHER_REGS) e = cudaErrorInvalidConfiguration;
+        if (e != cudaSuccess) return e;
+        ready = true;
+    }
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+    return launch_kernel(k, dim3((unsigned)p.n_items * G), A_THREADS, smem, 1, p.dependent & DEPENDENT_ATTENTION, stream, p, qm, km, vm);
+}
+
+template <typename T>
+cudaError_t launch_type(const DraftParams& p, cudaStream_t stream) {
+    if (p.d_key == 128) return p.d_value == 128 ? launch<T, 128, 128>(p, stream) : launch<T, 128, 64>(p, stream);
+    return p.d_value == 128 ? launch<T, 64, 128>(p, stream) : launch<T, 64, 64>(p, stream);
+}
+
+}  // namespace
+
+bool draft_tc_serves(const Geometry& g, int d_key, int d_value, int group, float scale) {
+    auto whole = [](int d) { return d == 64 || d == 128; };
+    return g.esize == 2 && g.chunk_size == A_TOK && whole(d_key) && whole(d_value) && group <= A_ROWS && scale != 0.f;
+}
+
+cudaError_t launch_draft_tc(const DraftParams& p, int dtype, cudaStream_t stream) {
+    return dtype == CA_DTYPE_F16 ? launch_type<__half>(p, stream) : launch_type<__nv_bfloat16>(p, stream);
+}
+
+}  // namespace ca

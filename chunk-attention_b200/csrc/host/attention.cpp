@@ -615,16 +615,27 @@ torch::Tensor Attention::forward_draft(torch::Tensor q, torch::Tensor k, torch::
         draft_version_ = tree_->version();
         draft_appended_ = tree_->appended();
     }
+    // The kernels of 16-bit caches take operands by tensor copies: whole 16-byte units, no stride of zero.  Others are laid out anew.  A dimension
+    // of one element may have any stride.
+    auto laid_out = [&](torch::Tensor& t, int64_t& node, int64_t& head) {
+        const int64_t d = t.size(2);
+        auto strides = [&] {
+            head = t.size(1) > 1 ? t.stride(1) : d;
+            node = t.size(0) > 1 ? t.stride(0) : t.size(1) * d;
+        };
+        strides();
+        if (t.element_size() == 2 && (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || node % 8 || head % 8 || node <= 0 || head <= 0) && d % 8 == 0) {
+            t = t.clone(at::MemoryFormat::Contiguous);
+            strides();
+        }
+    };
     ca_draft_args a{};
+    laid_out(q, a.q_node, a.q_head);
+    laid_out(k, a.k_node, a.k_head);
+    laid_out(v, a.v_node, a.v_head);
     a.q = q.data_ptr();
     a.k = k.data_ptr();
     a.v = v.data_ptr();
-    a.q_node = q.stride(0);
-    a.q_head = q.stride(1);
-    a.k_node = k.stride(0);
-    a.k_head = k.stride(1);
-    a.v_node = v.stride(0);
-    a.v_head = v.stride(1);
     a.out = out.data_ptr();
     a.seen = draft.view(&captured_).seen;
     a.words = draft.words();
@@ -895,6 +906,8 @@ void Attention::set_option(int option, int64_t value) {
     check_rc(ca_context_set_option(ctx_, option, value), "set_option");
     valid_ = false;
     shared_plan_ = std::make_shared<SharedPlan>();  // its work lists now differ from its siblings'
+    shared_draft_ = std::make_shared<std::shared_ptr<DraftWork>>();
+    draft_ = nullptr;
 }
 
 void Attention::attn_partials(torch::Tensor q, int phases) {

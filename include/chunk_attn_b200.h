@@ -163,6 +163,9 @@ CA_API int ca_context_create_shaped(ca_context** out, int device, const ca_head_
  * of 64 or 128 elements), in one launch instead of partial results and their combination: 1 (default) where that is faster, 0 never,
  * 2 always. */
 #define CA_OPT_DIRECT 12
+/* Attention of drafted trees, 16-bit caches of 64-token chunks and heads of 64 or 128 elements: 1 (default) the tcgen05 kernel, 0 the
+ * any-geometry one. */
+#define CA_OPT_DRAFT_TENSOR 15
 /* Failure-path tests only: the CTA that draws item `value` of the next launches (portions of prompts on tcgen05: piece
  * `value`, key/value heads fastest) stops feeding its consumer warps, whose bounded wait then runs out (status 1; portions:
  * 1 or 2).  -1 (default) switches it off. */

@@ -59,13 +59,20 @@ def test_values_of_hidden_nodes_do_not_matter(dtype, d):
     """Infinities and NaN in the keys and values of nodes show in the nodes below them only."""
     c = D.Case(7, dtype, 2, 2 if dtype == BF16 else 1, d, own=(70, 65), trees=[[-1, 0, 0, 1, 2, 3], [-1, 0, 1]])
     clean = c.run()
+    want = c.expected()
+    tol = c.tolerance(want)
+
+    def as_clean(out, rows):
+        # rows beside something infinite may be computed in another order: both ways are within the tolerance of the exact result
+        assert ((out.double() - want).abs() <= tol)[rows].all()
+
     for poison in (math.nan, math.inf):
         for t in (c.vd, c.kd):
             keep = t[2].clone()
             t[2] = poison  # node 2 of the first tree; node 4 is below it
             out = c.run()
-            rest = [0, 1, 3, 5, 6, 7, 8]
-            assert torch.equal(out[rest], clean[rest])
+            as_clean(out, [0, 1, 3, 5, 6, 7, 8])
+            assert torch.equal(out[6:], clean[6:])  # another tree
             assert not torch.isfinite(out[2]).any() and not torch.isfinite(out[4]).any()
             t[2] = keep
     c.vd[2, 0, 3] = math.inf  # a single element
@@ -73,7 +80,8 @@ def test_values_of_hidden_nodes_do_not_matter(dtype, d):
     group = c.H // c.G
     assert torch.isinf(out[2, :group, 3]).all() and torch.isinf(out[4, :group, 3]).all()
     out[[2, 4], :group, 3] = clean[[2, 4], :group, 3]
-    assert torch.equal(out, clean)
+    as_clean(out, list(range(9)))
+    assert torch.equal(out[:, group:], clean[:, group:])  # other heads
 
 
 @pytest.mark.parametrize("dtype,group,d", [(F16, 1, 128), (BF16, 4, 128), (F32, 1, 64)])
@@ -95,6 +103,19 @@ def test_strided_operands(dtype, group, d):
     assert torch.equal(c.cache.forward_draft(*odd, c.draft), want)
     one = c.kd[:1].expand(n, G, d)  # the same keys for all nodes
     assert torch.equal(c.cache.forward_draft(c.qd, one, c.vd, c.draft), c.cache.forward_draft(c.qd, one.contiguous(), c.vd, c.draft))
+
+
+@pytest.mark.parametrize("dtype,group,dk,dv", [(F16, 1, 128, 128), (BF16, 4, 64, 128), (BF16, 8, 128, 64)])
+def test_both_kernels(dtype, group, dk, dv):
+    """The any-geometry kernel serves what the tensor-core kernel does."""
+    from chunk_attn import cabi
+    c = D.Case(16, dtype, 2, group, dk, dv, shared=128, own=(300, 64, 5), nodes=(30, 4, 9))
+    a = c.check()
+    c.cache.set_option(cabi.CA_OPT_DRAFT_TENSOR, 0)
+    b = c.check()
+    assert not torch.equal(a, b)  # sums in another order: it is another kernel
+    c.cache.set_option(cabi.CA_OPT_DRAFT_TENSOR, 1)
+    assert torch.equal(a, c.run())
 
 
 def test_empty_drafts():
