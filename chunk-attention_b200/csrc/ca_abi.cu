@@ -1901,12 +1901,14 @@ int ca_accept_draft(const ca_accept_args* a, ca_stream stream) {
 // ---- log probabilities ---------------------------------------------------------------------------------------------------------
 int64_t ca_log_probs_scratch(int n_rows, int vocab, int dtype, int top) {
     if (n_rows < 0 || vocab < 1 || top < 0 || top > CA_MAX_TOP || !shaped_esize_of(dtype)) return -1;
-    return (int64_t)n_rows * sizeof(float2);
+    const bool stretches = ca::log_probs_splits(n_rows, vocab, shaped_esize_of(dtype)) == 0;
+    return (int64_t)n_rows * sizeof(float2) + (stretches ? ((int64_t)n_rows + ca::log_probs_ctas()) * (int64_t)sizeof(ca::LogProbsPart) : 0);
 }
 
 int ca_token_log_probs(const ca_log_probs_args* a, ca_stream stream) {
     if (!a) return fail(CA_ERR_INVALID, "null argument");
     if (a->n_rows < 0 || a->n_tokens < 0 || a->vocab < 1) return fail(CA_ERR_INVALID, "token_log_probs: bad sizes");
+    if (a->vocab > (1 << 28)) return fail(CA_ERR_INVALID, "token_log_probs: more than 2^28 tokens");
     if (!shaped_esize_of(a->dtype)) return fail(CA_ERR_INVALID, "token_log_probs: fp16, bf16 and fp32 only");
     if (a->top < 0 || a->top > CA_MAX_TOP || a->top > a->vocab) return fail(CA_ERR_INVALID, "token_log_probs: top must be 0 to 32 and not above the vocabulary");
     if (a->row_stride < 0) return fail(CA_ERR_INVALID, "token_log_probs: negative stride");
@@ -1918,8 +1920,7 @@ int ca_token_log_probs(const ca_log_probs_args* a, ca_stream stream) {
     p.row_stride = a->row_stride;
     p.n_rows = a->n_rows;
     p.vocab = a->vocab;
-    p.splits = ca::log_probs_splits(a->n_rows, a->vocab);
-    if ((int64_t)p.n_rows * p.splits > INT32_MAX) return fail(CA_ERR_INVALID, "token_log_probs: too many rows");
+    ca::log_probs_shape(p, shaped_esize_of(a->dtype));
     p.tokens = a->tokens;
     p.rows = a->rows;
     p.n_tokens = a->n_tokens;
@@ -1929,6 +1930,8 @@ int ca_token_log_probs(const ca_log_probs_args* a, ca_stream stream) {
     p.top_log_probs = a->top_log_probs;
     p.top_ids = a->top_ids;
     p.lse = static_cast<float2*>(a->scratch);
+    p.parts = reinterpret_cast<ca::LogProbsPart*>(p.lse + a->n_rows);
+    p.tokens_here = a->n_rows > 0 && (!a->rows || a->n_tokens <= 1024);  // every row's CTA reads the rows of all tokens
     CA_CUDA(ca::launch_log_probs(p, a->dtype, static_cast<cudaStream_t>(stream)));
     return CA_OK;
 }

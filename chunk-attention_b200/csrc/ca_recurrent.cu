@@ -12,6 +12,7 @@
 
 #include "../../include/chunk_attn_b200.h"
 #include "ca_kernels.h"
+#include "ca_logits.h"
 #include "ca_types.cuh"
 
 namespace ca {
@@ -1085,7 +1086,8 @@ int ca_selective_scan(void* y, const void* x, const void* z, int64_t z_stride, c
 
 int ca_block_status(int32_t* status, ca_stream stream) {
     if (!status) return fail("block_status: null pointer");
-    const cudaError_t e = read_decay_status(status, static_cast<cudaStream_t>(stream));
+    cudaError_t e = read_decay_status(status, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess && *status == STATUS_OK) e = read_log_probs_status(status, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? CA_OK : fail(cudaGetErrorString(e), CA_ERR_CUDA);
 }
 

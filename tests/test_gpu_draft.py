@@ -355,6 +355,18 @@ def test_log_probs(dtype, n, vocab, top):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("n,vocab,top", [(2000, 40, 3), (1999, 5001, 9), (100, 150001, 20), (601, 16384, 32), (130, 131077, 0)])
+def test_log_probs_of_many_rows(dtype, n, vocab, top):
+    """Rows that are cut between CTAs, and CTAs that have several rows."""
+    x = torch.randn(n, vocab, device=DEV, generator=torch.Generator(DEV).manual_seed(5)) * 3
+    x[n // 2] = -math.inf
+    x[n // 2, vocab // 3] = 1.0
+    x[n // 3] = 0.25
+    x[1, -1] = math.nan
+    check_log_probs(x.to(dtype), top)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_log_probs_of_odd_rows(dtype):
     """Rows that start at any address, and rows of a wider buffer."""
     buf = (torch.randn(9, 5003, device=DEV) * 4).to(dtype)
