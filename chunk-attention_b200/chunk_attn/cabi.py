@@ -214,8 +214,8 @@ class DraftPlan:
         check(lib.ca_draft_plan_data(self._h, C.byref(ptr), C.byref(self.info)))
         i = self.info
         data = np.ctypeslib.as_array(ptr, shape=(i.n_data,)).copy() if i.n_data else np.zeros(0, np.int32)
-        # items: first node, nodes, list, tiles, slot, first node of the tree, drafted nodes seen, tokens
-        self.items = data[:8 * i.n_items].reshape(-1, 8)
+        # items: first node, nodes, list, tiles, slot, first node of the tree, drafted nodes seen, tokens, the first four tiles
+        self.items = data[:16 * i.n_items].reshape(-1, 16)
         self.tiles = data[i.at_tiles:i.at_nodes]
         self.merge_nodes = data[i.at_nodes:i.at_nodes + i.n_merge]
         self.merge_off = data[i.at_off:i.at_off + i.n_merge + 1]

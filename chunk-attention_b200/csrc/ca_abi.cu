@@ -1809,7 +1809,7 @@ int ca_draft_attention(ca_context* c, const ca_draft_args* a, ca_stream stream_)
     if (reinterpret_cast<uintptr_t>(a->out) % 16 || reinterpret_cast<uintptr_t>(a->work) % 16 || reinterpret_cast<uintptr_t>(a->seen) % 8 ||
         reinterpret_cast<uintptr_t>(a->partials) % 16)
         return fail(CA_ERR_INVALID, "drafted tokens: out, work list and scratch must be 16-byte aligned");
-    if ((int64_t)a->info->n_items * c->geo.n_heads > INT32_MAX) return fail(CA_ERR_INVALID, "drafted tokens: too many pieces of work");
+    if ((int64_t)a->info->n_items * c->geo.n_heads > INT32_MAX || (int64_t)a->info->n_nodes * c->geo.n_heads * c->group > INT32_MAX - 4) return fail(CA_ERR_INVALID, "drafted tokens: too many pieces of work");
     DeviceGuard guard(c->device);
     if (guard.err != cudaSuccess) return fail_cuda(guard.err, "cudaSetDevice");
     const int H = c->geo.n_heads * c->group;

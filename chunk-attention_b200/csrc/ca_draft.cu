@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
     const int kvh = blockIdx.x % G;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 ia = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G)), ib = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 1);
-    const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w};
+    const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w, {}};
     if (!draft_item_ok(p, ia, ib, G_WARPS * RW)) {
         if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
         return;
@@ -256,60 +256,81 @@ cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t st
 }
 
 // ---- combination: a warp for every (node, query head) that several items serve ---------------------------------------------------
+// Its latency is all there is to it: which partial results a node has is read while the kernel before still runs (the work list has long been
+// there), and their rows are requested together with the maxima and sums, eight at a time.
 template <typename T, int COLS>
 __global__ void __launch_bounds__(128) draft_merge_kernel(const DraftParams p) {
+    constexpr int BATCH = COLS == 1 ? 8 : 4;
     const int H = p.geo.n_heads * p.group, lane = threadIdx.x & 31;
-    const int64_t pair = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int pair = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (pair >= p.n_merge * H) return;
+    const int i = pair / H, head = pair % H;
+    const int node = p.merge_nodes[i], b = p.merge_off[i], n = p.merge_off[i + 1] - b;
+    int slot = lane < n ? p.merge_slots[b + lane] : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (pair >= (int64_t)p.n_merge * H) return;
-    const int i = (int)(pair / H), head = (int)(pair % H);
-    const int node = p.merge_nodes[i], b = p.merge_off[i], e = p.merge_off[i + 1];
-    float M = p.sink ? 0.f : G_NEG_BIG;
-    for (int s = b + lane; s < e; s += 32) M = fmaxf(M, p.part_ml[(int64_t)p.merge_slots[s] * H + head].x);
-    M = warp_max(M);
-    float total = 0.f, o[COLS * 4];
+    float M = p.sink ? 0.f : G_NEG_BIG, total = 0.f, o[COLS * 4];
 #pragma unroll
     for (int c = 0; c < COLS * 4; c++) o[c] = 0.f;
-    for (int s0 = b; s0 < e; s0 += 32) {
+    for (int s0 = 0; s0 < n; s0 += 32) {
+        if (s0 > 0) slot = s0 + lane < n ? p.merge_slots[b + s0 + lane] : 0;
+        const int here = min(32, n - s0);
+        const int64_t at = (int64_t)slot * H + head;
+        const float2 ml = lane < here ? p.part_ml[at] : make_float2(G_NEG_BIG, 0.f);
         float w = 0.f;
-        int slot = 0;
-        if (s0 + lane < e) {
-            slot = p.merge_slots[s0 + lane];
-            const float2 ml = p.part_ml[(int64_t)slot * H + head];
-            w = exp2f(ml.x - M);
-            total += ml.y * w;
-        }
-        for (int k = 0; k < min(32, e - s0); k++) {
-            const float wk = __shfl_sync(0xffffffffu, w, k);
-            const float* from = p.part_o + ((int64_t)__shfl_sync(0xffffffffu, slot, k) * H + head) * p.part_width;
+        for (int k0 = 0; k0 < here; k0 += BATCH) {
+            float4 v[BATCH][COLS];
 #pragma unroll
-            for (int c = 0; c < COLS; c++) {
-                const int at = 128 * c + 4 * lane;
-                if (at >= p.part_width) continue;
-                const float4 v = *reinterpret_cast<const float4*>(from + at);
-                o[4 * c] = fmaf(wk, v.x, o[4 * c]);
-                o[4 * c + 1] = fmaf(wk, v.y, o[4 * c + 1]);
-                o[4 * c + 2] = fmaf(wk, v.z, o[4 * c + 2]);
-                o[4 * c + 3] = fmaf(wk, v.w, o[4 * c + 3]);
+            for (int k = 0; k < BATCH; k++) {
+                const int64_t from = __shfl_sync(0xffffffffu, at, min(k0 + k, here - 1)) * p.part_width;
+#pragma unroll
+                for (int c = 0; c < COLS; c++) {
+                    const int e = 128 * c + 4 * lane;
+                    v[k][c] = k0 + k < here && e < p.part_width ? *reinterpret_cast<const float4*>(p.part_o + from + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+            if (k0 == 0) {
+                const float high = fmaxf(M, warp_max(ml.x)), alpha = exp2f(M - high);
+                M = high;
+                w = exp2f(ml.x - M);
+                total = total * alpha + ml.y * w;  // this lane's pieces
+#pragma unroll
+                for (int c = 0; c < COLS * 4; c++) o[c] *= alpha;
+            }
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                const float wk = __shfl_sync(0xffffffffu, w, min(k0 + k, 31));
+                if (k0 + k >= here) continue;
+#pragma unroll
+                for (int c = 0; c < COLS; c++) {
+                    o[4 * c] = fmaf(wk, v[k][c].x, o[4 * c]);
+                    o[4 * c + 1] = fmaf(wk, v[k][c].y, o[4 * c + 1]);
+                    o[4 * c + 2] = fmaf(wk, v[k][c].z, o[4 * c + 2]);
+                    o[4 * c + 3] = fmaf(wk, v[k][c].w, o[4 * c + 3]);
+                }
             }
         }
     }
     total = warp_sum(total);
     if (p.sink) total += exp2f(-M);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
     T* out = static_cast<T*>(p.out) + ((int64_t)node * H + head) * p.d_value;
 #pragma unroll
-    for (int c = 0; c < COLS; c++)
+    for (int c = 0; c < COLS; c++) {
+        const int e = 128 * c + 4 * lane;
+        if (p.d_value % 4 == 0) {
+            if (e < p.d_value) *reinterpret_cast<Pack<T, 4>*>(out + e) = {from_f32<T>(o[4 * c] * inv), from_f32<T>(o[4 * c + 1] * inv), from_f32<T>(o[4 * c + 2] * inv), from_f32<T>(o[4 * c + 3] * inv)};
+        } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int at = 128 * c + 4 * lane + k;
-            if (at < p.d_value) out[at] = from_f32<T>(total == 0.f ? 0.f : o[4 * c + k] / total);
+            for (int k = 0; k < 4; k++)
+                if (e + k < p.d_value) out[e + k] = from_f32<T>(o[4 * c + k] * inv);
         }
+    }
 }
 
 template <typename T>
 cudaError_t merge(const DraftParams& p, cudaStream_t stream) {
-    const int64_t pairs = (int64_t)p.n_merge * p.geo.n_heads * p.group;
+    const int pairs = p.n_merge * p.geo.n_heads * p.group;
     const dim3 grid((unsigned)((pairs + 3) / 4));
     if (p.part_width <= 128) return launch_kernel(&draft_merge_kernel<T, 1>, grid, 128, 0, 1, p.dependent & DEPENDENT_MERGE, stream, p);
     return launch_kernel(&draft_merge_kernel<T, 2>, grid, 128, 0, 1, p.dependent & DEPENDENT_MERGE, stream, p);

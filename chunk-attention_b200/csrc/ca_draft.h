@@ -29,8 +29,9 @@ struct DraftItem {
     int32_t slot;            // partial results go to slots slot .. slot + n_nodes - 1; -1: finished rows are stored
     int32_t tree, n_drafted; // first node of the row's tree and how many of its nodes the block may see; 0: none
     int32_t tokens;          // of all its tiles
+    int32_t head[8];         // its first four {pool slot, tokens} pairs once more: a CTA's first copies need not wait for the list
 };
-static_assert(sizeof(DraftItem) == 32, "DraftItem is read on the device as two int4");
+static_assert(sizeof(DraftItem) == 64, "DraftItem is read on the device as four int4");
 
 struct DraftPlan {
     std::vector<DraftItem> items;  // longest first

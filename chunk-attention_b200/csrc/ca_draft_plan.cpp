@@ -119,6 +119,10 @@ std::string build_draft_plan(DraftPlan& plan, const ca_chunk_info* infos, int n_
                 it.tree = u.tree;
                 it.n_drafted = ui >= n_runs && pc == pieces - 1 ? it.node0 + it.n_nodes - u.tree : 0;
                 for (int c = c0; c < c1; c++) it.tokens += u.tiles[2 * c + 1];
+                for (int c = c0; c < std::min(c1, c0 + 4); c++) {
+                    it.head[2 * (c - c0)] = u.tiles[2 * c];
+                    it.head[2 * (c - c0) + 1] = u.tiles[2 * c + 1];
+                }
                 it.slot = -1;
                 if (pieces > 1 || served[u.node0] > 1) {
                     it.slot = plan.n_slots;

@@ -38,7 +38,7 @@ using namespace ptx;
 constexpr int A_ROWS = 128, A_TOK = 64, A_SLOTS = 4, A_THREADS = 256;
 constexpr int A_SOFTMAX_REGS = 200, A_OTHER_REGS = 56;  // per thread; the block is launched with 2 x 128 (checked at the launch)
 constexpr int A_TMEM_COLS = 256, A_COL_S = 128;
-constexpr int A_NUM_BARS = 2 * A_SLOTS + 13;
+constexpr int A_NUM_BARS = 2 * A_SLOTS + 14;
 constexpr float A_NEG_BIG = -1.0e30f, A_RESCALE_STEP = 8.f;
 
 template <typename T> __host__ __device__ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
@@ -73,6 +73,7 @@ struct alignas(16) Work {
     int node0, n_rows, n_tiles, n_context;  // tiles in all, and from the pool
     int list, tree, n_drafted, slot;
     int n_nodes, kvh, pad[2];
+    int2 head[4];  // the first tiles of the pool: slot, tokens
 };
 
 template <int DK, int DV> struct Sizes {
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
     const uint32_t q_full = o_free + 8;
     const uint32_t q_empty = q_full + 8;
     const uint32_t clc_bar = q_empty + 8;
+    const uint32_t ask_bar = clc_bar + 8;
     Work* const work = reinterpret_cast<Work*>(smem + Z::WORK);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Z::BARS + A_NUM_BARS * 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -173,6 +175,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
         mbar_init(clc_bar, 1);
+        mbar_init(ask_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 5) {  // the warp that allocates is the warp that frees
@@ -183,8 +186,8 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
     __syncthreads();
     tc_fence_after_thread_sync();
     const uint32_t tmem_base = *tmem_slot;
-    // with tensor memory in hand: a kernel behind this one may allocate, too
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // with tensor memory in hand: a kernel behind this one may allocate, too.  Only the producer waits for the kernels before: the work list and the
+    // trees' bits have long been there (they came by copies, which no kernel overtakes), and what is stored follows from what is loaded.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // a wait of a single thread: false, with the code recorded, when the limit ran out
     auto wait = [&](uint32_t bar, int parity, int code) {
@@ -196,11 +199,12 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
     if (warp >= 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(A_OTHER_REGS));
         if (warp == 6 && lane == 0) {
-            // ---- the next piece of work, asked for when the piece before the present one is finished
+            // ---- the next piece of work, asked for when the present one's last tiles are: a CTA that starts early, while the kernel before drains, must
+            // not take what others will soon be there for (asked for at once, a wave of single pieces took twice its time back to back)
             int item = blockIdx.x;
             for (int n = 0;; n++) {
                 if (n > 0) {
-                    if (!wait(work_empty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, STATUS_EMPTY_WAIT_TIMEOUT)) break;
+                    if (!wait(ask_bar, (n - 1) & 1, STATUS_EMPTY_WAIT_TIMEOUT) || !wait(work_empty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, STATUS_EMPTY_WAIT_TIMEOUT)) break;
                     mbar_arrive_expect_tx(clc_bar, 16);
                     clc_try_cancel(sbase + Z::CLC, clc_bar);
                     if (!wait(clc_bar, (n - 1) & 1, STATUS_FULL_WAIT_TIMEOUT)) {
@@ -213,7 +217,11 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                 Work w{};
                 if (item >= 0) {
                     const int4* it = reinterpret_cast<const int4*>(p.items + item / G);
-                    const int4 a = __ldg(it), b = __ldg(it + 1);
+                    const int4 a = __ldg(it), b = __ldg(it + 1), c = __ldg(it + 2), d = __ldg(it + 3);
+                    w.head[0] = make_int2(c.x, c.y);
+                    w.head[1] = make_int2(c.z, c.w);
+                    w.head[2] = make_int2(d.x, d.y);
+                    w.head[3] = make_int2(d.z, d.w);
                     w.node0 = a.x;
                     w.n_nodes = a.y;
                     w.n_rows = a.y * group;
@@ -237,15 +245,21 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
         } else if (warp == 4 && lane == 0) {
             // ---- producer: slot i & 3 takes K of tile i / 2 (even i) or its V (odd i), i counted over all pieces
             int issued = 0, q_issued = 0, n = 0;
+            asm volatile("griddepcontrol.wait;" ::: "memory");
             for (bool live = true; live; n++) {
                 if (!wait(work_full + 8 * (n & 1), (n >> 1) & 1, STATUS_FULL_WAIT_TIMEOUT)) break;
                 const Work w = work[n & 1];
                 mbar_arrive(work_empty + 8 * (n & 1));
                 if (w.n_tiles == 0) break;
                 const int2* tiles = reinterpret_cast<const int2*>(p.tiles) + w.list;
-                int2 tile = w.n_context > 0 ? __ldg(tiles) : make_int2(0, 0);
+                // asked for four tiles ahead: on its way while slots are waited for
+                int2 queue[4] = {w.head[0], w.head[1], w.head[2], w.head[3]};
                 for (int j = 0; j < w.n_tiles && live; j++) {
-                    const int2 next = j + 1 < w.n_context ? __ldg(tiles + j + 1) : make_int2(0, 0);  // on its way while slots are waited for
+                    int2 tile = queue[0];
+                    queue[0] = queue[1];
+                    queue[1] = queue[2];
+                    queue[2] = queue[3];
+                    queue[3] = j + 4 < w.n_context ? __ldg(tiles + j + 4) : make_int2(0, 0);
                     if (j < w.n_context && (tile.x < 0 || tile.x >= p.max_chunks || tile.y <= 0 || tile.y > A_TOK)) {
                         report(p.status, STATUS_BAD_WORK_LIST);  // keep the pipeline moving on a chunk that exists
                         tile = make_int2(0, A_TOK);
@@ -274,6 +288,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                                 tma_load_3d(dst + pn * (A_TOK * 128), side ? &v_map : &k_map, 64 * pn, w.kvh, w.tree + (j - w.n_context) * A_TOK, bar);
                         }
                         issued++;
+                        if (side == 0 && j == max(0, w.n_tiles - 3)) mbar_arrive(ask_bar);
                         if (j == 0 && side == 0) {
                             // the queries follow the first K tile.  Rows past the block are other nodes' or zeros: nobody reads theirs
                             if (!wait(q_empty, (n & 1) ^ 1, STATUS_EMPTY_WAIT_TIMEOUT)) {
@@ -286,7 +301,6 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                             q_issued++;
                         }
                     }
-                    tile = next;
                 }
             }
             for (int f = issued > A_SLOTS ? issued - A_SLOTS : 0; f < issued; f++)
@@ -295,7 +309,9 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
         } else if (warp == 5 && elect_one()) {
             // ---- MMA issuer: one thread; t counts tiles over all pieces
             constexpr uint32_t DESC_HI = umma_desc_sw128_hi(1024);
-            constexpr uint32_t IDESC_QK = idesc_of<T>(A_TOK, false), IDESC_PV = idesc_of<T>(DV, true);
+            // a negative scale: the products of the negated queries (bit 13), so that the largest score stays the largest
+            const uint32_t idesc_qk = idesc_of<T>(A_TOK, false) | (p.scale_log2 < 0.f ? 1u << 13 : 0u);
+            constexpr uint32_t IDESC_PV = idesc_of<T>(DV, true);
             const uint32_t q_lo = umma_desc_sw128_lo(sbase, 16);
             auto issue_qk = [&](int t) {
                 const int i = 2 * t, slot = i & (A_SLOTS - 1);
@@ -307,7 +323,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                 for (int ks = 0; ks < DK / 16; ks++) {
                     const uint64_t a = umma_desc_pack(q_lo + (((ks >> 2) * Z::Q_PANEL + (ks & 3) * 32) >> 4), DESC_HI);
                     const uint64_t b = umma_desc_pack(b_lo + (((ks >> 2) * (A_TOK * 128) + (ks & 3) * 32) >> 4), DESC_HI);
-                    umma_ss_f16(d, a, b, IDESC_QK, ks > 0 ? 1u : 0u);
+                    umma_ss_f16(d, a, b, idesc_qk, ks > 0 ? 1u : 0u);
                 }
                 umma_commit(s_full + 8 * (t & 1));
                 umma_commit(empty_bar + 8 * slot);
@@ -351,8 +367,6 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(A_SOFTMAX_REGS));
         // ---- softmax: thread r owns query row r = TMEM lane r
         const int r = threadIdx.x;
-        // a negative scale: the largest score is then that of the negated product
-        const uint32_t flip = p.scale_log2 < 0.f ? 0x80000000u : 0u;
         const float scale = fabsf(p.scale_log2);
         const uint32_t lane_addr = tmem_base + ((uint32_t)(warp * 32) << 16);
         uint8_t* const stage = smem + Z::OUT + warp * 32 * Z::OUT_PITCH;
@@ -374,7 +388,8 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
             for (int j = 0; j < w.n_tiles; j++, t++) {
                 const int b = t & 1;
                 const bool drafted = j >= w.n_context;
-                const int filled = drafted ? min(A_TOK, w.n_drafted - (j - w.n_context) * A_TOK) : max(0, min(A_TOK, __ldg(p.tiles + 2 * (w.list + j) + 1)));
+                const int stored = drafted ? 0 : (j == 0 ? w.head[0].y : __ldg(p.tiles + 2 * (w.list + j) + 1));
+                const int filled = drafted ? min(A_TOK, w.n_drafted - (j - w.n_context) * A_TOK) : max(0, min(A_TOK, stored));
                 uint2 see = make_uint2(0u, 0u);
                 if (drafted) see = __ldg(line + (j - w.n_context));
                 if (!(live = wait_all(s_full + 8 * b, (t >> 1) & 1))) break;
@@ -386,13 +401,6 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                     tmem_ld32(lane_addr + A_COL_S + b * A_TOK, s0);
                     tmem_ld32(lane_addr + A_COL_S + b * A_TOK + 32, s1);
                     tmem_wait_ld();
-                    if (flip) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            s0[i] ^= flip;
-                            s1[i] ^= flip;
-                        }
-                    }
                     if (drafted || filled < A_TOK) {
                         if (!drafted) {
                             see.x = filled >= 32 ? 0xffffffffu : (1u << filled) - 1;
@@ -452,9 +460,11 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
             }
             if (!live || !(live = wait_all(o_done, (t - 1) & 1))) break;
             tc_fence_after_thread_sync();
-            // ---- epilogue: finished rows as 16-bit elements, 32 columns at a time through the warp's own shared memory; partial rows as
-            // fp32, 16 columns at a time.  Sums of 0 x show whether an x is not finite.
+            // ---- epilogue: rows are stored finished (16 bits) or partial (fp32).  Sums of 0 x show whether an x is not finite.
             float scale_out = 1.f, check = 0.f;
+            const int64_t row_bytes = w.slot < 0 ? DV * 2 : p.part_width * 4;
+            char* const base = (w.slot < 0 ? static_cast<char*>(p.out) : reinterpret_cast<char*>(p.part_o)) + (int64_t)(w.slot < 0 ? w.node0 : w.slot) * H * row_bytes;
+            auto row_at = [&](int row) { return base + ((int64_t)(row / group) * H + w.kvh * group + row % group) * row_bytes; };
             if (w.slot < 0) {
                 float total = l, M = m_used;
                 if (p.sink) {
@@ -465,15 +475,14 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
             } else if (active) {
                 p.part_ml[(int64_t)(w.slot + my_node - w.node0) * H + w.kvh * group + r % group] = make_float2(m_used, l);
             }
+            // Up to 16 rows: a thread stores its own.  More: 32 columns (partial: 16) of a warp's rows at a time through shared memory, four lanes
+            // to a row (128 rows straight from the threads: 15.6 us instead of 14.2 for one wave of pieces of two tiles; 13 rows through
+            // shared memory: 9.7 instead of 9.0)
+            const bool straight = w.n_rows <= 16;
             const int rows_here = min(32, w.n_rows - warp * 32);
-            char* to[4];  // four lanes to a row
-            const int64_t row_bytes = w.slot < 0 ? DV * 2 : p.part_width * 4;
+            char* to[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int row = warp * 32 + 8 * k + (lane >> 2), at = row / group, head = w.kvh * group + row % group;
-                char* base = w.slot < 0 ? static_cast<char*>(p.out) : reinterpret_cast<char*>(p.part_o);
-                to[k] = base + ((int64_t)((w.slot < 0 ? w.node0 : w.slot) + at) * H + head) * row_bytes + 16 * (lane & 3);
-            }
+            for (int k = 0; k < 4; k++) to[k] = straight ? row_at(r) : row_at(warp * 32 + 8 * k + (lane >> 2)) + 16 * (lane & 3);
             // A loop, not unrolled: this code runs once a piece, and straight through it the warps waited for instructions
 #pragma unroll 1
             for (int c = 0; c < DV / 32; c++) {
@@ -496,6 +505,14 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     if (half == 1 && w.slot < 0) break;
+                    const int at = w.slot < 0 ? 64 * c : 128 * c + 64 * half;
+                    if (straight) {
+                        if (active) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(to[0] + at + 16 * i) = make_uint4(o[16 * half + 4 * i], o[16 * half + 4 * i + 1], o[16 * half + 4 * i + 2], o[16 * half + 4 * i + 3]);
+                        }
+                        continue;
+                    }
                     __syncwarp();  // what was staged before has been read
 #pragma unroll
                     for (int i = 0; i < 4; i++)
@@ -505,10 +522,11 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                     for (int k = 0; k < 4; k++) {
                         const int rr = 8 * k + (lane >> 2);
                         const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * Z::OUT_PITCH + 16 * (lane & 3));
-                        if (rr < rows_here) *reinterpret_cast<uint4*>(to[k] + (w.slot < 0 ? 64 * c : 128 * c + 64 * half)) = v;
+                        if (rr < rows_here) *reinterpret_cast<uint4*>(to[k] + at) = v;
                     }
                 }
             }
+            __syncwarp();
             const uint32_t again = __ballot_sync(0xffffffffu, active && !(check + 0.f * l == 0.f));
             if (again) {
                 __syncwarp();  // the rows above have been stored

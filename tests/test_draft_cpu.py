@@ -45,7 +45,8 @@ def walk(plan, infos, trees, q, kd, vd, pool, G, group):
     part, written = {}, set()
     line = sum((D.lines(t) for t in trees), [])
     row_of = [r for r, t in enumerate(trees) for _ in t]
-    for node0, n_nodes, lst, n_tiles, slot, tree, n_drafted, tokens in plan.items.tolist():
+    for node0, n_nodes, lst, n_tiles, slot, tree, n_drafted, tokens, *head in plan.items.tolist():
+        assert head[:2 * n_tiles] == plan.tiles[2 * lst:2 * (lst + min(4, n_tiles))].tolist()
         assert n_nodes >= 1 and n_nodes * group <= max(plan.info.block_rows, group)
         keys, vals, ids = [], [], []
         for j in range(n_tiles):
