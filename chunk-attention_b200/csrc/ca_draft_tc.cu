@@ -158,6 +158,9 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Z::BARS + A_NUM_BARS * 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.geo.n_heads, group = p.group, H = G * group;
+    // rows to nodes: r / group for r < 128 by a product (the quotient's fraction is 1 / group at least, the product is off by r / 65536 at most)
+    const uint32_t by_group = (65536u + group - 1) / group;
+    auto node_of = [&](int row) { return (int)((uint32_t)row * by_group >> 16); };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < A_SLOTS; i++) {
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
             const Work w = work[n & 1];
             if (w.n_tiles == 0) break;
             const bool active = r < w.n_rows, busy = warp * 32 < w.n_rows;
-            const int my_node = w.node0 + (active ? r / group : 0);
+            const int my_at = active ? node_of(r) : 0, my_node = w.node0 + my_at;
             const uint2* line = reinterpret_cast<const uint2*>(p.seen + (int64_t)my_node * p.words);
             float m_used = A_NEG_BIG, l = 0.f;
             for (int j = 0; j < w.n_tiles; j++, t++) {
@@ -442,16 +445,12 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                         tmem_st32(lane_addr + c * 32, o);
                     }
                 }
-                if (filled < A_TOK) {
-                    // The rows of V behind the tokens meet weights of zero, so they only have to be finite.  Of a pool tile they are not
-                    // copied (the slot's earlier tile, whose MMA of tile t - 2 is complete, may be another sequence's); of a drafted
-                    // one they are other trees', and are overwritten once the tile is there.
-                    const int vi = 2 * t + 1;
-                    if (drafted && !(live = wait_all(full_bar + 8 * (vi & (A_SLOTS - 1)), (vi / A_SLOTS) & 1))) break;
-                    const uint32_t v_slot = ring + (vi & (A_SLOTS - 1)) * Z::SLOT;
-                    const int grans = (A_TOK - filled) * 8;
-                    for (int i = r; i < (DV / 64) * grans; i += 4 * 32)
-                        sts128_zero(v_slot + (i / grans) * (A_TOK * 128) + filled * 128 + (i % grans) * 16);
+                if (!drafted && filled < A_TOK) {
+                    // The rows of V behind the tokens meet weights of zero, so they only have to be finite.  They are not copied: the slot's earlier
+                    // tile, whose MMA of tile t - 2 is complete, may be another sequence's.  (A drafted tile's are other trees' or zeros.)
+                    constexpr int PER_LINE = DV / 8;  // 16-byte granules of a row, 8 to a panel
+                    const uint32_t to = ring + ((2 * t + 1) & (A_SLOTS - 1)) * Z::SLOT + ((r % PER_LINE) >> 3) * (A_TOK * 128) + (r & 7) * 16;
+                    for (int t_line = filled + r / PER_LINE; t_line < A_TOK; t_line += 4 * 32 / PER_LINE) sts128_zero(to + t_line * 128);
                     fence_proxy_async();
                 }
                 tmem_wait_st();
@@ -461,10 +460,13 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
             if (!live || !(live = wait_all(o_done, (t - 1) & 1))) break;
             tc_fence_after_thread_sync();
             // ---- epilogue: rows are stored finished (16 bits) or partial (fp32).  Sums of 0 x show whether an x is not finite.
-            float scale_out = 1.f, check = 0.f;
+            float scale_out = 1.f, check[4] = {0.f, 0.f, 0.f, 0.f};
             const int64_t row_bytes = w.slot < 0 ? DV * 2 : p.part_width * 4;
             char* const base = (w.slot < 0 ? static_cast<char*>(p.out) : reinterpret_cast<char*>(p.part_o)) + (int64_t)(w.slot < 0 ? w.node0 : w.slot) * H * row_bytes;
-            auto row_at = [&](int row) { return base + ((int64_t)(row / group) * H + w.kvh * group + row % group) * row_bytes; };
+            auto row_at = [&](int row) {
+                const int at = node_of(row);
+                return base + (int64_t)(at * H + w.kvh * group + row - at * group) * row_bytes;
+            };
             if (w.slot < 0) {
                 float total = l, M = m_used;
                 if (p.sink) {
@@ -473,7 +475,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                 }
                 scale_out = total == 0.f ? 0.f : fast_exp2(m_used - M) / total;
             } else if (active) {
-                p.part_ml[(int64_t)(w.slot + my_node - w.node0) * H + w.kvh * group + r % group] = make_float2(m_used, l);
+                p.part_ml[(int64_t)(w.slot + my_at) * H + w.kvh * group + r - my_at * group] = make_float2(m_used, l);
             }
             // Up to 16 rows: a thread stores its own.  More: 32 columns (partial: 16) of a warp's rows at a time through shared memory, four lanes
             // to a row (128 rows straight from the threads: 15.6 us instead of 14.2 for one wave of pieces of two tiles; 13 rows through
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
             const int rows_here = min(32, w.n_rows - warp * 32);
             char* to[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) to[k] = straight ? row_at(r) : row_at(warp * 32 + 8 * k + (lane >> 2)) + 16 * (lane & 3);
+            for (int k = 0; k < 4; k++) to[k] = straight ? (k == 0 ? row_at(r) : nullptr) : row_at(warp * 32 + 8 * k + (lane >> 2)) + 16 * (lane & 3);
             // A loop, not unrolled: this code runs once a piece, and straight through it the warps waited for instructions
 #pragma unroll 1
             for (int c = 0; c < DV / 32; c++) {
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                 }
                 if (!busy) continue;
 #pragma unroll
-                for (int i = 0; i < 32; i++) check = fmaf(0.f, __uint_as_float(o[i]), check);
+                for (int i = 0; i < 32; i++) check[i & 3] = fmaf(0.f, __uint_as_float(o[i]), check[i & 3]);
                 if (w.slot < 0) {
 #pragma unroll
                     for (int i = 0; i < 16; i++) o[i] = pack2<T>(__uint_as_float(o[2 * i]) * scale_out, __uint_as_float(o[2 * i + 1]) * scale_out);
@@ -527,7 +529,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                 }
             }
             __syncwarp();
-            const uint32_t again = __ballot_sync(0xffffffffu, active && !(check + 0.f * l == 0.f));
+            const uint32_t again = __ballot_sync(0xffffffffu, active && !(check[0] + check[1] + check[2] + check[3] + 0.f * l == 0.f));
             if (again) {
                 __syncwarp();  // the rows above have been stored
                 for (uint32_t rest = again; rest; rest &= rest - 1) row_again<T>(p, w, warp * 32 + __ffs(rest) - 1, lane);
