@@ -459,8 +459,9 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
             }
             if (!live || !(live = wait_all(o_done, (t - 1) & 1))) break;
             tc_fence_after_thread_sync();
-            // ---- epilogue: rows are stored finished (16 bits) or partial (fp32).  Sums of 0 x show whether an x is not finite.
-            float scale_out = 1.f, check[4] = {0.f, 0.f, 0.f, 0.f};
+            // ---- epilogue: rows are stored finished (16 bits) or partial (fp32).  Their sum shows whether an element is not finite.
+            float scale_out = 1.f;
+            uint64_t check = 0;
             const int64_t row_bytes = w.slot < 0 ? DV * 2 : p.part_width * 4;
             char* const base = (w.slot < 0 ? static_cast<char*>(p.out) : reinterpret_cast<char*>(p.part_o)) + (int64_t)(w.slot < 0 ? w.node0 : w.slot) * H * row_bytes;
             auto row_at = [&](int row) {
@@ -499,10 +500,14 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                 }
                 if (!busy) continue;
 #pragma unroll
-                for (int i = 0; i < 32; i++) check[i & 3] = fmaf(0.f, __uint_as_float(o[i]), check[i & 3]);
+                for (int i = 0; i < 16; i++) check = add_f32x2(check, pair_u32(o[2 * i], o[2 * i + 1]));
                 if (w.slot < 0) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = pack2<T>(__uint_as_float(o[2 * i]) * scale_out, __uint_as_float(o[2 * i + 1]) * scale_out);
+                    for (int i = 0; i < 16; i++) {
+                        float a, bb;
+                        unpair_f32(mul_f32x2(pair_u32(o[2 * i], o[2 * i + 1]), pair_f32(scale_out, scale_out)), a, bb);
+                        o[i] = pack2<T>(a, bb);
+                    }
                 }
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
@@ -529,7 +534,9 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                 }
             }
             __syncwarp();
-            const uint32_t again = __ballot_sync(0xffffffffu, active && !(check[0] + check[1] + check[2] + check[3] + 0.f * l == 0.f));
+            float sum_a, sum_b;
+            unpair_f32(check, sum_a, sum_b);
+            const uint32_t again = __ballot_sync(0xffffffffu, active && !(fabsf(sum_a) + fabsf(sum_b) + l < INFINITY));
             if (again) {
                 __syncwarp();  // the rows above have been stored
                 for (uint32_t rest = again; rest; rest &= rest - 1) row_again<T>(p, w, warp * 32 + __ffs(rest) - 1, lane);
