@@ -1765,7 +1765,7 @@ int ca_draft_plan_for_context(const ca_context* c, ca_draft_plan** out, const ca
         shape.ctas = 2 * ca::B200_SMS;
     } else {
         shape.block_rows = ca::draft_generic_rows(std::min(widest, 64) * c->group);
-        shape.ctas = 4 * ca::B200_SMS;
+        shape.ctas = ca::draft_generic_ctas(shape.block_rows, c->shaped ? c->shape.d_key : c->geo.d_head, c->shaped ? c->shape.d_value : c->geo.d_head, c->geo.esize);
     }
     if (c->group > 64) return fail(CA_ERR_INVALID, "drafted tokens: more than 64 query heads to a key/value head");
     return make_draft_plan(out, infos, n_infos, first, n_rows, shape);
@@ -1861,6 +1861,11 @@ int ca_draft_attention(ca_context* c, const ca_draft_args* a, ca_stream stream_)
         CA_CUDA(ca::launch_draft_merge(p, c->dtype, stream));
         return CA_OK;
     }
+    const int es = c->geo.esize;
+    auto whole = [&](const void* t, int64_t node, int64_t head, int d) {
+        return reinterpret_cast<uintptr_t>(t) % 16 == 0 && node * es % 16 == 0 && head * es % 16 == 0 && d * es % 16 == 0;
+    };
+    p.whole_granules = whole(a->k, a->k_node, a->k_head, p.d_key) && whole(a->v, a->v_node, a->v_head, p.d_value);
     CA_CUDA(ca::launch_draft_generic(p, a->info->block_rows, c->dtype, stream));
     CA_CUDA(ca::launch_draft_merge(p, c->dtype, stream));
     return CA_OK;

@@ -10,55 +10,210 @@
 #include "ca_draft.h"
 #include "ca_kernels.h"
 #include "ca_launch.cuh"
+#include "ca_ptx.cuh"
 #include "ca_types.cuh"
 
 namespace ca {
 namespace {
 
-constexpr int G_THREADS = 128, G_WARPS = 4, G_TOK = 32;
+constexpr int G_THREADS = 128, G_WARPS = 4, G_TOK = 32, G_STAGES = 2;
 constexpr float G_NEG_BIG = -1.0e30f;
 
-__host__ __device__ constexpr int round4(int x) { return (x + 3) & ~3; }
-// floats between rows in shared memory: whole 16-byte granules, an odd number of them, so that 8 lanes reading a granule each of
-// consecutive rows meet no bank twice
-__host__ __device__ constexpr int pitch_of(int d) { return round4(d) + ((round4(d) / 4) % 2 == 0 ? 4 : 0); }
+__host__ __device__ constexpr int whole(int x, int unit) { return (x + unit - 1) / unit * unit; }
+struct GenericSizes {
+    int k_bytes, v_bytes, q_floats;  // of a key and a value as staged, of a query row
+    __host__ __device__ int stage() const { return G_TOK * (k_bytes + v_bytes); }
+};
+__host__ __device__ inline GenericSizes generic_sizes(int dk, int dv, int esize) { return {whole(dk * esize, 16), whole(dv * esize, 16), whole(dk, 16 / esize)}; }
+// Byte of granule g of token t of a staged tile: as the pool has it, 128-byte panels of which the granules of a line are XORed with the token (so
+// neither eight tokens' like granules nor a token's granules meet a bank twice), or rows
+__device__ __forceinline__ int staged(int t, int g, int row_bytes, int swz) { return swz ? ((g >> 3) * G_TOK + t) * 128 + (((g & 7) ^ (t & 7)) << 4) : t * row_bytes + g * 16; }
 
-// One element of a stored tile as fp32
-template <typename T> __device__ __forceinline__ float pool_elem(const T* tile, const Geometry& side, int t, int e) {
-    return to_f32(tile[tile_elem_offset(side, t, e)]);
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// An item for one key/value head.  Four warps with RW query rows each (row r: query head r % group of node r / group); the keys go by in tiles
-// of 32 tokens, staged as fp32.  Scores: a lane has a token, and multiplies its key with the warp's rows (read by all lanes at once).
-// Softmax: over the lanes.  Output: a lane has the columns 4 lane .. 4 lane + 3 of each 128, weights come from shared memory.
+// The tiles of an item: parts of chunks of up to 32 tokens, then of the row's tree
+struct Tile { int chunk, first, n; };  // chunk < 0: drafted; n = 0: there is none
+template <typename T> struct Walk {
+    static constexpr int E = 16 / sizeof(T);
+    const DraftParams& p;
+    const GenericSizes& z;
+    const DraftItem& it;
+    const int kvh;
+    uint8_t* const stages;
+    int j = 0, t0 = 0, d0 = 0, chunk = -1, in_chunk = 0;
+    __device__ __forceinline__ Walk(const DraftParams& p, const GenericSizes& z, const DraftItem& it, int kvh, uint8_t* stages) : p(p), z(z), it(it), kvh(kvh), stages(stages) {}
+    __device__ __forceinline__ Tile take() {
+        while (j < it.n_tiles) {
+            if (t0 == 0) {
+                const int2 e = __ldg(reinterpret_cast<const int2*>(p.tiles) + it.list + j);
+                chunk = e.x;
+                in_chunk = e.y;
+                if (chunk < 0 || chunk >= p.max_chunks || in_chunk > p.geo.chunk_size) {
+                    if (threadIdx.x == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
+                    in_chunk = 0;
+                }
+            }
+            if (t0 >= in_chunk) {
+                j++;
+                t0 = 0;
+                continue;
+            }
+            const Tile t = {chunk, t0, min(G_TOK, in_chunk - t0)};
+            t0 += G_TOK;
+            return t;
+        }
+        const Tile t = {-1, d0, max(0, min(G_TOK, it.n_drafted - d0))};
+        d0 += G_TOK;
+        return t;
+    }
+    // By a whole block.  Parts of chunks whose rows are whole granules by bulk copies of thread 0, which complete on the stage's barrier (true);
+    // drafted rows of whole granules by asynchronous copies, others by plain ones.  Lines behind the tile's tokens hold anything.
+    __device__ __forceinline__ bool fetch(const Tile& t, int stage, uint32_t bar) const {
+        uint8_t* const sk = stages + stage * z.stage();
+        uint8_t* const sv = sk + G_TOK * z.k_bytes;
+        const uint32_t to_k = (uint32_t)__cvta_generic_to_shared(sk), to_v = (uint32_t)__cvta_generic_to_shared(sv);
+        if (t.chunk >= 0 && p.geo.epg == E) {
+            if (threadIdx.x == 0) {
+                const uint8_t* kt = static_cast<const uint8_t*>(p.pool) + tile_base_elems(p.geo, t.chunk, kvh, 0) * (int)sizeof(T);
+                const uint8_t* vt = kt + p.geo.tile_elems * (int)sizeof(T);
+                ptx::mbar_arrive_expect_tx(bar, t.n * (z.k_bytes + z.v_bytes));
+                auto side = [&](uint32_t to, const uint8_t* from, int row_bytes, int swz) {
+                    if (swz) {
+                        for (int pn = 0; pn < row_bytes / 128; pn++)
+                            ptx::bulk_copy_g2s(to + pn * (G_TOK * 128), from + ((int64_t)pn * p.geo.chunk_size + t.first) * 128, t.n * 128, bar);
+                    } else {
+                        ptx::bulk_copy_g2s(to, from + (int64_t)t.first * row_bytes, t.n * row_bytes, bar);
+                    }
+                };
+                side(to_k, kt, z.k_bytes, p.geo.swz);
+                side(to_v, vt, z.v_bytes, p.geo.v_swz);
+            }
+            return true;
+        }
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        if (t.chunk < 0 && p.whole_granules) {
+            auto side = [&](uint32_t to, const void* base, int64_t node, int64_t head, int row_bytes, int swz) {
+                const T* from = static_cast<const T*>(base) + (int64_t)(it.tree + t.first + warp) * node + (int64_t)kvh * head;
+                for (int g = lane; g < row_bytes / 16; g += 32)
+#pragma unroll
+                    for (int i = 0; i < G_TOK / G_WARPS; i++)
+                        if (warp + G_WARPS * i < t.n) cp_async16(to + staged(warp + G_WARPS * i, g, row_bytes, swz), from + i * G_WARPS * node + g * E);
+            };
+            side(to_k, p.k, p.k_node, p.k_head, z.k_bytes, p.geo.swz);
+            side(to_v, p.v, p.v_node, p.v_head, z.v_bytes, p.geo.v_swz);
+        } else {
+            auto side = [&](uint8_t* to, const T* from, int d, int row_bytes, int swz, const Geometry& g, int64_t node) {
+                for (int x = warp; x < t.n; x += G_WARPS)
+#pragma unroll 4
+                    for (int e = lane; e < row_bytes / (int)sizeof(T); e += 32) {
+                        const T v = e < d ? (t.chunk >= 0 ? from[tile_elem_offset(g, t.first + x, e)] : from[x * node + e]) : from_f32<T>(0.f);
+                        reinterpret_cast<T*>(to + staged(x, e / E, row_bytes, swz))[e % E] = v;
+                    }
+            };
+            const T *kt, *vt;
+            if (t.chunk >= 0) {
+                kt = static_cast<const T*>(p.pool) + tile_base_elems(p.geo, t.chunk, kvh, 0);
+                vt = kt + p.geo.tile_elems;
+            } else {
+                kt = static_cast<const T*>(p.k) + (int64_t)(it.tree + t.first) * p.k_node + (int64_t)kvh * p.k_head;
+                vt = static_cast<const T*>(p.v) + (int64_t)(it.tree + t.first) * p.v_node + (int64_t)kvh * p.v_head;
+            }
+            side(sk, kt, p.d_key, z.k_bytes, p.geo.swz, tile_side(p.geo, 0), p.k_node);
+            side(sv, vt, p.d_value, z.v_bytes, p.geo.v_swz, tile_side(p.geo, 1), p.v_node);
+        }
+        return false;
+    }
+};
+
+// What both kernels do around a tile: the stages' barriers, the wait for one
+struct Stages {
+    uint32_t bars, used = 0, phases = 0;  // bits: the stage's tile comes by bulk copies, the phase its barrier is in
+    long long limit;
+    int* status;
+    template <typename T> __device__ __forceinline__ void fetch(const Walk<T>& walk, const Tile& t, int stage) {
+        const bool bulk = walk.fetch(t, stage, bars + 8 * stage);
+        used = (used & ~(1u << stage)) | (bulk ? 1u << stage : 0u);
+    }
+    // The tile of the stage is there, for the whole block.  False: a copy did not come in time; status is recorded
+    __device__ __forceinline__ bool wait(int stage) {
+        bool ok = true;
+        if ((used >> stage) & 1) {
+            ok = ptx::mbar_wait_bounded(bars + 8 * stage, (phases >> stage) & 1, limit);
+            phases ^= 1u << stage;
+        } else {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+        if (__syncthreads_and(ok)) return true;
+        if (threadIdx.x == 0) {
+            atomicCAS(status, STATUS_OK, STATUS_FULL_WAIT_TIMEOUT);
+            if (!ptx::mbar_wait_bounded(bars + 8 * stage, ((phases >> stage) & 1) ^ 1, limit)) atomicCAS(status, STATUS_OK, STATUS_DRAIN_TIMEOUT);
+        }
+        return false;
+    }
+};
+__device__ __forceinline__ Stages make_stages(const DraftParams& p, uint64_t* bars) {
+    Stages s;
+    s.bars = (uint32_t)__cvta_generic_to_shared(bars);
+    s.limit = p.wait_limit;
+    s.status = p.status;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < G_STAGES; i++) ptx::mbar_init(s.bars + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    return s;
+}
+// Query rows row, row + step, ... of an item to shared memory as fp32, their loads side by side
+template <typename T, int ROWS> __device__ __forceinline__ void stage_queries(const DraftParams& p, const DraftItem& it, int kvh, float* sq, int q_floats, int n_rows, int row, int step) {
+    const int lane = threadIdx.x & 31;
+    const T* from[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const int r = min(row + step * i, n_rows - 1), at = r / p.group;
+        from[i] = static_cast<const T*>(p.q) + (int64_t)(it.node0 + at) * p.q_node + (int64_t)(kvh * p.group + r - at * p.group) * p.q_head;
+    }
+    for (int e0 = lane; e0 < q_floats; e0 += 128) {
+        float x[4][ROWS];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) x[k][i] = e0 + 32 * k < p.d_key ? to_f32(from[i][e0 + 32 * k]) : 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int i = 0; i < ROWS; i++)
+                if (e0 + 32 * k < q_floats) sq[(row + step * i) * q_floats + e0 + 32 * k] = x[k][i];
+    }
+}
+
+// An item for one key/value head.  Four warps with RW query rows each (row r: query head r % group of node r / group); the keys go by in tiles of
+// 32 tokens, staged as they are, the next one on its way.  Scores: a lane has a token, and multiplies its key with the warp's rows (read by all
+// lanes at once).  Softmax: over the lanes, the rows' steps side by side.  Output: a lane has the columns 4 lane .. 4 lane + 3 of each 128,
+// weights come from shared memory.  For 17 rows and more; bound by fp32 products and the reads that feed them.
 template <typename T, int RW, int COLS>  // COLS: groups of 128 value columns
-__global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftParams p) {
-    extern __shared__ __align__(16) float smem[];
-    const int dk = p.d_key, dv = p.d_value, kp = pitch_of(dk), vp = COLS * 128;
-    float* const sq = smem;                              // [4 RW][kp]
-    float* const sk = sq + G_WARPS * RW * kp;            // [32][kp]
-    float* const sv = sk + G_TOK * kp;                   // [32][vp]
-    float* const sp = sv + G_TOK * vp;                   // [4 RW][32] weights
+__global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftParams p, const GenericSizes z) {
+    extern __shared__ __align__(128) uint8_t raw[];
+    __shared__ uint64_t bars[G_STAGES];
+    constexpr int E = 16 / sizeof(T);
+    float* const sq = reinterpret_cast<float*>(raw);     // [4 RW][q_floats]
+    float* const sp = sq + G_WARPS * RW * z.q_floats;    // [4 RW][32] weights
+    uint8_t* const stages = raw + whole((int)sizeof(float) * G_WARPS * RW * (z.q_floats + G_TOK), 128);
+    const int dk = p.d_key, dv = p.d_value, stage_bytes = z.stage();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int G = p.geo.n_heads, group = p.group, H = G * group, C = p.geo.chunk_size;
+    const int G = p.geo.n_heads, group = p.group, H = G * group;
     const int kvh = blockIdx.x % G;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 ia = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G)), ib = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 1);
     const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w, {}};
     if (!draft_item_ok(p, ia, ib, G_WARPS * RW)) {
         if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
         return;
     }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int n_rows = it.n_nodes * group;
-
-    for (int i = tid; i < G_WARPS * RW * kp; i += G_THREADS) {
-        const int r = i / kp, e = i % kp;
-        float x = 0.f;
-        if (r < n_rows && e < dk)
-            x = to_f32(static_cast<const T*>(p.q)[(int64_t)(it.node0 + r / group) * p.q_node + (int64_t)(kvh * group + r % group) * p.q_head + e]);
-        sq[i] = x;
-    }
+    const int n_rows = it.n_nodes * group, row0 = warp * RW;
+    const bool busy = row0 < n_rows;
+    const int k_gran = whole(dk, E) / E, v_gran = whole(dv, E) / E;  // of a staged row
+    Walk<T> tiles(p, z, it, kvh, stages);
     float m[RW], l[RW], o[RW][COLS * 4];
 #pragma unroll
     for (int r = 0; r < RW; r++) {
@@ -67,35 +222,56 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
 #pragma unroll
         for (int c = 0; c < COLS * 4; c++) o[r][c] = 0.f;
     }
-    const int row0 = warp * RW;
-    const bool busy = row0 < n_rows;
-    const Geometry k_side = tile_side(p.geo, 0), v_side = tile_side(p.geo, 1);
-
-    // scores, softmax and output of the staged tile: n tokens, and for drafted ones which of them a row sees
-    auto work = [&](int n, bool drafted, int word, int shift) {
-        __syncthreads();
+    Stages in = make_stages(p, bars);
+    // the work list is old; what it names is the kernels' before
+    Tile now = tiles.take();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (now.n > 0) in.fetch(tiles, now, 0);
+#pragma unroll
+    for (int half = 0; half < RW; half += 4) stage_queries<T, 4>(p, it, kvh, sq, z.q_floats, n_rows, row0 + half, 1);
+    for (int stage = 0; now.n > 0; stage ^= 1) {
+        if (!in.wait(stage)) return;  // nobody reads the tile before this one any more
+        const Tile after = tiles.take();
+        if (after.n > 0) in.fetch(tiles, after, stage ^ 1);
         if (busy) {
+            const uint8_t* const sk = stages + stage * stage_bytes;
+            const uint8_t* const sv = sk + G_TOK * z.k_bytes;
+            const bool drafted = now.chunk < 0;
             float s[RW];
 #pragma unroll
             for (int r = 0; r < RW; r++) s[r] = 0.f;
-            for (int e = 0; e < dk; e += 4) {
-                const float4 k = *reinterpret_cast<const float4*>(sk + lane * kp + e);
+#pragma unroll 2
+            for (int g = 0; g < k_gran; g++) {
+                float k[E];
+                Granule<T>::load(reinterpret_cast<const T*>(sk + staged(lane, g, z.k_bytes, p.geo.swz)), k);
 #pragma unroll
-                for (int r = 0; r < RW; r++) {
-                    const float4 q = *reinterpret_cast<const float4*>(sq + (row0 + r) * kp + e);
-                    s[r] = fmaf(q.x, k.x, s[r]);
-                    s[r] = fmaf(q.y, k.y, s[r]);
-                    s[r] = fmaf(q.z, k.z, s[r]);
-                    s[r] = fmaf(q.w, k.w, s[r]);
-                }
+                for (int r = 0; r < RW; r++)
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        const float4 q = *reinterpret_cast<const float4*>(sq + (row0 + r) * z.q_floats + g * E + e);
+                        s[r] = fmaf(q.x, k[e], s[r]);
+                        s[r] = fmaf(q.y, k[e + 1], s[r]);
+                        s[r] = fmaf(q.z, k[e + 2], s[r]);
+                        s[r] = fmaf(q.w, k[e + 3], s[r]);
+                    }
             }
+            uint32_t line[RW];  // tokens of the tile that a row sees
+            float high[RW];
 #pragma unroll
             for (int r = 0; r < RW; r++) {
-                bool see = lane < n && row0 + r < n_rows;
-                if (drafted && see) see = (p.seen[(int64_t)(it.node0 + (row0 + r) / group) * p.words + word] >> (shift + lane)) & 1;
-                const float x = see ? s[r] * p.scale_log2 : -INFINITY;
-                const float mn = fmaxf(m[r], warp_max(x));
-                const float alpha = exp2f(m[r] - mn), w = see ? exp2f(x - mn) : 0.f;
+                line[r] = now.n == 32 ? 0xffffffffu : (1u << now.n) - 1;
+                if (drafted) line[r] &= __ldg(p.seen + (int64_t)(it.node0 + min(row0 + r, n_rows - 1) / group) * p.words + now.first / 32);
+                s[r] = (line[r] >> lane) & 1 ? s[r] * p.scale_log2 : -INFINITY;
+                high[r] = s[r];
+            }
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1)
+#pragma unroll
+                for (int r = 0; r < RW; r++) high[r] = fmaxf(high[r], __shfl_xor_sync(0xffffffffu, high[r], off));
+#pragma unroll
+            for (int r = 0; r < RW; r++) {
+                const float mn = fmaxf(m[r], high[r]), alpha = exp2_approx(m[r] - mn), w = (line[r] >> lane) & 1 ? exp2_approx(s[r] - mn) : 0.f;
                 m[r] = mn;
                 l[r] = l[r] * alpha + w;  // this lane's tokens only: summed over the lanes at the end
                 sp[(row0 + r) * G_TOK + lane] = w;
@@ -105,118 +281,69 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
                 }
             }
             __syncwarp();
-            if (!drafted) {
+            auto value = [&](int t, int c, float (&v)[4]) {  // columns 128 c + 4 lane ...
+                if (128 * c + 4 * lane < v_gran * E) {
+                    const int e = 128 * c + 4 * lane;
+                    const Pack<T, 4> x = *reinterpret_cast<const Pack<T, 4>*>(sv + staged(t, e / E, z.v_bytes, p.geo.v_swz) + e % E * (int)sizeof(T));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = to_f32(x.v[i]);
+                } else {
+                    v[0] = v[1] = v[2] = v[3] = 0.f;
+                }
+            };
+            if (!drafted && now.n == G_TOK) {
 #pragma unroll 1
                 for (int t = 0; t < G_TOK; t += 4) {
-                    float4 v[4][COLS];
+                    float v[4][COLS][4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
+                    for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int c = 0; c < COLS; c++) v[j][c] = *reinterpret_cast<const float4*>(sv + (t + j) * vp + 128 * c + 4 * lane);
+                        for (int c = 0; c < COLS; c++) value(t + i, c, v[i][c]);
 #pragma unroll
                     for (int r = 0; r < RW; r++) {
                         const float4 w4 = *reinterpret_cast<const float4*>(sp + (row0 + r) * G_TOK + t);
                         const float w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
+                        for (int i = 0; i < 4; i++)
 #pragma unroll
-                            for (int c = 0; c < COLS; c++) {
-                                o[r][4 * c] = fmaf(w[j], v[j][c].x, o[r][4 * c]);
-                                o[r][4 * c + 1] = fmaf(w[j], v[j][c].y, o[r][4 * c + 1]);
-                                o[r][4 * c + 2] = fmaf(w[j], v[j][c].z, o[r][4 * c + 2]);
-                                o[r][4 * c + 3] = fmaf(w[j], v[j][c].w, o[r][4 * c + 3]);
-                            }
+                            for (int c = 0; c < COLS; c++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) o[r][4 * c + e] = fmaf(w[i], v[i][c][e], o[r][4 * c + e]);
                     }
                 }
             } else {
-                // values of nodes that a row does not see may be infinite: they are left out, not multiplied by zero
+                // values that a row does not see may be infinite: they are left out, not multiplied by zero
 #pragma unroll 1
-                for (int t = 0; t < n; t++)
+                for (int t = 0; t < now.n; t++) {
+                    float v[COLS][4];
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) value(t, c, v[c]);
 #pragma unroll
                     for (int r = 0; r < RW; r++) {
-                        const bool see = row0 + r < n_rows && (p.seen[(int64_t)(it.node0 + (row0 + r) / group) * p.words + word] >> (shift + t)) & 1;
-                        if (!see) continue;
                         const float w = sp[(row0 + r) * G_TOK + t];
+                        if (!((line[r] >> t) & 1)) continue;
 #pragma unroll
-                        for (int c = 0; c < COLS; c++) {
-                            const float4 v = *reinterpret_cast<const float4*>(sv + t * vp + 128 * c + 4 * lane);
-                            o[r][4 * c] = fmaf(w, v.x, o[r][4 * c]);
-                            o[r][4 * c + 1] = fmaf(w, v.y, o[r][4 * c + 1]);
-                            o[r][4 * c + 2] = fmaf(w, v.z, o[r][4 * c + 2]);
-                            o[r][4 * c + 3] = fmaf(w, v.w, o[r][4 * c + 3]);
-                        }
+                        for (int c = 0; c < COLS; c++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[r][4 * c + e] = fmaf(w, v[c][e], o[r][4 * c + e]);
                     }
-            }
-        }
-        __syncthreads();
-    };
-
-    for (int j = 0; j < it.n_tiles; j++) {
-        int chunk = p.tiles[2 * (it.list + j)];
-        const int in_chunk = p.tiles[2 * (it.list + j) + 1];
-        if (chunk < 0 || chunk >= p.max_chunks || in_chunk > C) {
-            if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
-            continue;
-        }
-        const T* kt = static_cast<const T*>(p.pool) + tile_base_elems(p.geo, chunk, kvh, 0);
-        const T* vt = kt + p.geo.tile_elems;
-        for (int t0 = 0; t0 < in_chunk; t0 += G_TOK) {
-            const int n = min(G_TOK, in_chunk - t0);
-            constexpr int E = 16 / sizeof(T);
-            if (p.geo.epg == E) {
-                for (int i = tid; i < G_TOK * p.geo.gpr; i += G_THREADS) {
-                    const int t = i / p.geo.gpr, g = i % p.geo.gpr;
-                    float x[E];
-#pragma unroll
-                    for (int e = 0; e < E; e++) x[e] = 0.f;
-                    if (t < n) Granule<T>::load(kt + tile_granule_index(p.geo, t0 + t, g) * E, x);
-#pragma unroll
-                    for (int e = 0; e < E; e += 4)
-                        if (g * E + e < kp) *reinterpret_cast<float4*>(sk + t * kp + g * E + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                }
-                for (int i = tid; i < G_TOK * p.geo.v_gpr; i += G_THREADS) {
-                    const int t = i / p.geo.v_gpr, g = i % p.geo.v_gpr;
-                    float x[E];
-#pragma unroll
-                    for (int e = 0; e < E; e++) x[e] = 0.f;
-                    if (t < n) Granule<T>::load(vt + tile_granule_index(v_side, t0 + t, g) * E, x);
-#pragma unroll
-                    for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(sv + t * vp + g * E + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                }
-            } else {
-                for (int i = tid; i < G_TOK * kp; i += G_THREADS) {
-                    const int t = i / kp, e = i % kp;
-                    sk[i] = t < n && e < dk ? pool_elem(kt, k_side, t0 + t, e) : 0.f;
-                }
-                for (int i = tid; i < G_TOK * dv; i += G_THREADS) {
-                    const int t = i / dv, e = i % dv;
-                    sv[t * vp + e] = t < n ? pool_elem(vt, v_side, t0 + t, e) : 0.f;
                 }
             }
-            work(n, false, 0, 0);
         }
-    }
-    for (int t0 = 0; t0 < it.n_drafted; t0 += G_TOK) {
-        const int n = min(G_TOK, it.n_drafted - t0);
-        for (int i = tid; i < G_TOK * kp; i += G_THREADS) {
-            const int t = i / kp, e = i % kp;
-            sk[i] = t < n && e < dk ? to_f32(static_cast<const T*>(p.k)[(int64_t)(it.tree + t0 + t) * p.k_node + (int64_t)kvh * p.k_head + e]) : 0.f;
-        }
-        for (int i = tid; i < G_TOK * dv; i += G_THREADS) {
-            const int t = i / dv, e = i % dv;
-            sv[t * vp + e] = t < n ? to_f32(static_cast<const T*>(p.v)[(int64_t)(it.tree + t0 + t) * p.v_node + (int64_t)kvh * p.v_head + e]) : 0.f;
-        }
-        work(n, true, t0 / 32, 0);
+        now = after;
     }
     if (!busy) return;
 #pragma unroll
+    for (int off = 16; off >= 1; off >>= 1)
+#pragma unroll
+        for (int r = 0; r < RW; r++) l[r] += __shfl_xor_sync(0xffffffffu, l[r], off);
+#pragma unroll
     for (int r = 0; r < RW; r++) {
-        const float sum = warp_sum(l[r]);
         if (row0 + r >= n_rows) continue;
         const int node = it.node0 + (row0 + r) / group, head = kvh * group + (row0 + r) % group;
         if (it.slot >= 0) {
             const int64_t at = (int64_t)(it.slot + node - it.node0) * H + head;
-            if (lane == 0) p.part_ml[at] = make_float2(m[r], sum);
+            if (lane == 0) p.part_ml[at] = make_float2(m[r], l[r]);
 #pragma unroll
             for (int c = 0; c < COLS; c++) {
                 const int e = 128 * c + 4 * lane;
@@ -224,35 +351,243 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
             }
         } else {
             const float M = p.sink ? fmaxf(m[r], 0.f) : m[r];
-            const float w = exp2f(m[r] - M), total = sum * w + (p.sink ? exp2f(-M) : 0.f);
+            const float w = exp2_approx(m[r] - M), total = l[r] * w + (p.sink ? exp2_approx(-M) : 0.f), scale = total == 0.f ? 0.f : w / total;
             T* out = static_cast<T*>(p.out) + ((int64_t)node * H + head) * dv;
 #pragma unroll
-            for (int c = 0; c < COLS; c++)
+            for (int c = 0; c < COLS; c++) {
+                const int e = 128 * c + 4 * lane;
+                if (dv % 4 == 0) {
+                    if (e < dv) *reinterpret_cast<Pack<T, 4>*>(out + e) = {from_f32<T>(o[r][4 * c] * scale), from_f32<T>(o[r][4 * c + 1] * scale), from_f32<T>(o[r][4 * c + 2] * scale), from_f32<T>(o[r][4 * c + 3] * scale)};
+                } else {
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int e = 128 * c + 4 * lane + k;
-                    if (e < dv) out[e] = from_f32<T>(total == 0.f ? 0.f : o[r][4 * c + k] * w / total);
+                    for (int k = 0; k < 4; k++)
+                        if (e + k < dv) out[e + k] = from_f32<T>(o[r][4 * c + k] * scale);
                 }
+            }
+        }
+    }
+}
+
+// The same for at most 16 rows (chains, small trees): the warps share the rows' work instead of the rows.  A warp multiplies a quarter of the
+// key's granules, the quarters meet in shared memory, where every row has its warp for the softmax, and a warp has a quarter of the value's
+// columns, a lane each.  (With a warp's rows its own, few rows leave three warps of every block idle and load one scheduler of the SM: one row
+// of 2000 tokens, 32 fp32 heads of 128, 4 nodes: 62 us.)
+template <typename T, int R, int COLS>  // COLS: columns of a lane
+__global__ void __launch_bounds__(G_THREADS) draft_few_kernel(const DraftParams p, const GenericSizes z) {
+    extern __shared__ __align__(128) uint8_t raw[];
+    __shared__ uint64_t bars[G_STAGES];
+    constexpr int E = 16 / sizeof(T), MINE = R / G_WARPS;  // rows of a warp in the softmax
+    float* const sq = reinterpret_cast<float*>(raw);     // [R][q_floats]
+    float* const ss = sq + R * z.q_floats;               // [4][R][32] quarters of scores
+    float* const sp = ss + G_WARPS * R * G_TOK;          // [R][32] weights
+    float* const sa = sp + R * G_TOK;                    // [R] what the rows' earlier results are scaled by
+    float2* const ml = reinterpret_cast<float2*>(sa + R);
+    uint8_t* const stages = raw + whole((int)sizeof(float) * R * (z.q_floats + (G_WARPS + 1) * G_TOK + 3), 128);
+    const int dk = p.d_key, dv = p.d_value;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = p.geo.n_heads, group = p.group, H = G * group;
+    const int kvh = blockIdx.x % G;
+    const int4 ia = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G)), ib = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 1);
+    const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w, {}};
+    if (!draft_item_ok(p, ia, ib, R)) {
+        if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
+        return;
+    }
+    const int n_rows = it.n_nodes * group, k_gran = whole(dk, E) / E;
+    Walk<T> tiles(p, z, it, kvh, stages);
+    Stages in = make_stages(p, bars);
+    Tile now = tiles.take();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (now.n > 0) in.fetch(tiles, now, 0);
+    stage_queries<T, MINE>(p, it, kvh, sq, z.q_floats, n_rows, warp, G_WARPS);
+    float m[MINE], l[MINE], o[R][COLS];
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+        m[i] = G_NEG_BIG;
+        l[i] = 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int c = 0; c < COLS; c++) o[r][c] = 0.f;
+    const int col0 = warp * 32 * COLS + lane;  // and 32 further
+    for (int stage = 0; now.n > 0; stage ^= 1) {
+        if (!in.wait(stage)) return;  // nobody reads the tile before this one any more
+        const Tile after = tiles.take();
+        if (after.n > 0) in.fetch(tiles, after, stage ^ 1);
+        const uint8_t* const sk = stages + stage * z.stage();
+        const uint8_t* const sv = sk + G_TOK * z.k_bytes;
+        auto value = [&](int t, int c) {
+            const int e = col0 + 32 * c;
+            return e < dv ? to_f32(*reinterpret_cast<const T*>(sv + staged(t, e / E, z.v_bytes, p.geo.v_swz) + e % E * (int)sizeof(T))) : 0.f;
+        };
+        const bool drafted = now.chunk < 0;
+        {
+            float s[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) s[r] = 0.f;
+#pragma unroll 2
+            for (int g = warp; g < k_gran; g += G_WARPS) {
+                float k[E];
+                Granule<T>::load(reinterpret_cast<const T*>(sk + staged(lane, g, z.k_bytes, p.geo.swz)), k);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        const float4 q = *reinterpret_cast<const float4*>(sq + r * z.q_floats + g * E + e);
+                        s[r] = fmaf(q.x, k[e], s[r]);
+                        s[r] = fmaf(q.y, k[e + 1], s[r]);
+                        s[r] = fmaf(q.z, k[e + 2], s[r]);
+                        s[r] = fmaf(q.w, k[e + 3], s[r]);
+                    }
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) ss[(warp * R + r) * G_TOK + lane] = s[r];
+        }
+        const uint32_t there = now.n == 32 ? 0xffffffffu : (1u << now.n) - 1;
+        __syncthreads();
+        {
+            float s[MINE], high[MINE];
+            bool see[MINE];
+#pragma unroll
+            for (int i = 0; i < MINE; i++) {
+                const int r = warp + G_WARPS * i;
+                uint32_t line = there;
+                if (drafted) line &= __ldg(p.seen + (int64_t)(it.node0 + min(r, n_rows - 1) / group) * p.words + now.first / 32);
+                see[i] = (line >> lane) & 1;
+                float x = 0.f;
+#pragma unroll
+                for (int w = 0; w < G_WARPS; w++) x += ss[(w * R + r) * G_TOK + lane];
+                s[i] = high[i] = see[i] ? x * p.scale_log2 : -INFINITY;
+            }
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1)
+#pragma unroll
+                for (int i = 0; i < MINE; i++) high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], off));
+#pragma unroll
+            for (int i = 0; i < MINE; i++) {
+                const int r = warp + G_WARPS * i;
+                const float mn = fmaxf(m[i], high[i]), alpha = exp2_approx(m[i] - mn), w = see[i] ? exp2_approx(s[i] - mn) : 0.f;
+                m[i] = mn;
+                l[i] = l[i] * alpha + w;  // this lane's tokens only
+                sp[r * G_TOK + lane] = w;
+                if (lane == 0) sa[r] = alpha;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float alpha = sa[r];
+#pragma unroll
+            for (int c = 0; c < COLS; c++) o[r][c] *= alpha;
+        }
+        if (!drafted && now.n == G_TOK) {
+#pragma unroll 2
+            for (int t = 0; t < G_TOK; t += 4) {
+                float v[4][COLS];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) v[i][c] = value(t + i, c);
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float4 w = *reinterpret_cast<const float4*>(sp + r * G_TOK + t);
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) {
+                        o[r][c] = fmaf(w.x, v[0][c], o[r][c]);
+                        o[r][c] = fmaf(w.y, v[1][c], o[r][c]);
+                        o[r][c] = fmaf(w.z, v[2][c], o[r][c]);
+                        o[r][c] = fmaf(w.w, v[3][c], o[r][c]);
+                    }
+                }
+            }
+        } else {
+            // values that a row does not see may be infinite: they are left out, not multiplied by zero
+            uint32_t line[R];
+            int node = it.node0, head = 0;
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                line[r] = drafted && r < n_rows ? there & __ldg(p.seen + (int64_t)node * p.words + now.first / 32) : there;
+                if (++head == group) {
+                    head = 0;
+                    node++;
+                }
+            }
+#pragma unroll 1
+            for (int t = 0; t < now.n; t++) {
+                float v[COLS];
+#pragma unroll
+                for (int c = 0; c < COLS; c++) v[c] = value(t, c);
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float w = sp[r * G_TOK + t];
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) o[r][c] = (line[r] >> t) & 1 ? fmaf(w, v[c], o[r][c]) : o[r][c];
+                }
+            }
+        }
+        now = after;
+    }
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+        const float sum = warp_sum(l[i]);
+        if (lane == 0) ml[warp + G_WARPS * i] = make_float2(m[i], sum);
+    }
+    __syncthreads();
+    int at_node = 0, in_group = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        if (r >= n_rows) break;
+        const int head = kvh * group + in_group;
+        const float2 own = ml[r];
+        if (it.slot >= 0) {
+            const int64_t at = (int64_t)(it.slot + at_node) * H + head;
+            if (tid == 0) p.part_ml[at] = own;
+#pragma unroll
+            for (int c = 0; c < COLS; c++)
+                if (col0 + 32 * c < p.part_width) p.part_o[at * p.part_width + col0 + 32 * c] = o[r][c];
+        } else {
+            const float M = p.sink ? fmaxf(own.x, 0.f) : own.x;
+            const float w = exp2_approx(own.x - M), total = own.y * w + (p.sink ? exp2_approx(-M) : 0.f), scale = total == 0.f ? 0.f : w / total;
+            T* out = static_cast<T*>(p.out) + ((int64_t)(it.node0 + at_node) * H + head) * dv;
+#pragma unroll
+            for (int c = 0; c < COLS; c++)
+                if (col0 + 32 * c < dv) out[col0 + 32 * c] = from_f32<T>(o[r][c] * scale);
+        }
+        if (++in_group == group) {
+            in_group = 0;
+            at_node++;
         }
     }
 }
 
 template <typename T>
 cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t stream) {
-    auto go = [&](auto* k, int rw, int cols) {
-        const size_t smem = sizeof(float) * ((size_t)(G_WARPS * rw + G_TOK) * pitch_of(p.d_key) + G_TOK * cols * 128 + G_WARPS * rw * G_TOK);
+    const GenericSizes z = generic_sizes(p.d_key, p.d_value, sizeof(T));
+    auto go = [&](auto* k, size_t floats) {
+        const size_t smem = whole((int)(sizeof(float) * floats), 128) + (size_t)G_STAGES * z.stage();
         cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         if (e != cudaSuccess) return e;
-        return launch_kernel(k, dim3((unsigned)p.n_items * p.geo.n_heads), G_THREADS, smem, 1, p.dependent & DEPENDENT_ATTENTION, stream, p);
+        return launch_kernel(k, dim3((unsigned)p.n_items * p.geo.n_heads), G_THREADS, smem, 1, p.dependent & DEPENDENT_ATTENTION, stream, p, z);
     };
-    if (p.geo.d_value <= 128 && p.d_value <= 128) {
-        if (block_rows <= 16) return go(&draft_generic_kernel<T, 4, 1>, 4, 1);
-        if (block_rows <= 32) return go(&draft_generic_kernel<T, 8, 1>, 8, 1);
-        return go(&draft_generic_kernel<T, 16, 1>, 16, 1);
+    auto few = [&](auto* k, int r) { return go(k, (size_t)r * (z.q_floats + (G_WARPS + 1) * G_TOK + 3)); };
+    auto many = [&](auto* k, int rw) { return go(k, (size_t)G_WARPS * rw * (z.q_floats + G_TOK)); };
+    if (p.d_value <= 128) {
+        if (block_rows <= 4) return few(&draft_few_kernel<T, 4, 1>, 4);
+        if (block_rows <= 8) return few(&draft_few_kernel<T, 8, 1>, 8);
+        if (block_rows <= 12) return few(&draft_few_kernel<T, 12, 1>, 12);
+        if (block_rows <= 16) return few(&draft_few_kernel<T, 16, 1>, 16);
+        if (block_rows <= 32) return many(&draft_generic_kernel<T, 8, 1>, 8);
+        return many(&draft_generic_kernel<T, 16, 1>, 16);
     }
-    if (block_rows <= 16) return go(&draft_generic_kernel<T, 4, 2>, 4, 2);
-    if (block_rows <= 32) return go(&draft_generic_kernel<T, 8, 2>, 8, 2);
-    return go(&draft_generic_kernel<T, 16, 2>, 16, 2);
+    if (block_rows <= 4) return few(&draft_few_kernel<T, 4, 2>, 4);
+    if (block_rows <= 8) return few(&draft_few_kernel<T, 8, 2>, 8);
+    if (block_rows <= 12) return few(&draft_few_kernel<T, 12, 2>, 12);
+    if (block_rows <= 16) return few(&draft_few_kernel<T, 16, 2>, 16);
+    if (block_rows <= 32) return many(&draft_generic_kernel<T, 8, 2>, 8);
+    return many(&draft_generic_kernel<T, 16, 2>, 16);
 }
 
 // ---- combination: a warp for every (node, query head) that several items serve ---------------------------------------------------
@@ -383,6 +718,12 @@ __global__ void __launch_bounds__(32) accept_draft_kernel(const AcceptParams p) 
 }
 
 }  // namespace
+
+int draft_generic_ctas(int block_rows, int dk, int dv, int esize) {
+    const GenericSizes z = generic_sizes(dk, dv, esize);
+    const int rows = sizeof(float) * block_rows * (z.q_floats + (block_rows <= 16 ? (G_WARPS + 1) * G_TOK + 3 : G_TOK));
+    return B200_SMS * std::max(1, std::min(4, 232448 / (rows + G_STAGES * z.stage() + 1024 + 128)));
+}
 
 cudaError_t launch_draft_generic(const DraftParams& p, int block_rows, int dtype, cudaStream_t stream) {
     if (dtype == CA_DTYPE_F32) return launch_generic<float>(p, block_rows, stream);

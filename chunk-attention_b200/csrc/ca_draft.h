@@ -62,6 +62,7 @@ struct DraftParams {
     int d_key, d_value;        // of q, k, v and out; the pool's may be padded
     const void *q, *k, *v;     // [n_nodes, heads, .]: element strides below, the last 1
     int64_t q_node, q_head, k_node, k_head, v_node, v_head;
+    bool whole_granules;       // addresses, strides and head sizes of k and v are whole 16-byte units
     void* out;                 // [n_nodes, heads, d_value]
     float scale_log2;          // scale * log2(e)
     int sink;
@@ -88,9 +89,10 @@ __device__ __forceinline__ bool draft_item_ok(const DraftParams& p, int4 a, int4
 }
 #endif
 // query rows of an item that the any-geometry kernel takes, for units of so many
-inline int draft_generic_rows(int unit_rows) { return unit_rows <= 16 ? 16 : (unit_rows <= 32 ? 32 : 64); }
+inline int draft_generic_rows(int unit_rows) { return unit_rows <= 4 ? 4 : (unit_rows <= 16 ? (unit_rows + 3) / 4 * 4 : (unit_rows <= 32 ? 32 : 64)); }
 
 #if defined(__CUDACC__)
+int draft_generic_ctas(int block_rows, int dk, int dv, int esize);  // that run at a time
 cudaError_t launch_draft_generic(const DraftParams& p, int block_rows, int dtype, cudaStream_t stream);
 bool draft_tc_serves(const Geometry& g, int d_key, int d_value, int group, float scale);
 cudaError_t launch_draft_tc(const DraftParams& p, int dtype, cudaStream_t stream);
