@@ -43,13 +43,15 @@ template <typename T> struct Walk {
     const int kvh;
     uint8_t* const stages;
     int j = 0, t0 = 0, d0 = 0, chunk = -1, in_chunk = 0;
-    __device__ __forceinline__ Walk(const DraftParams& p, const GenericSizes& z, const DraftItem& it, int kvh, uint8_t* stages) : p(p), z(z), it(it), kvh(kvh), stages(stages) {}
+    int2 next;  // chunk j's pair, asked for a chunk ahead
+    __device__ __forceinline__ int2 entry(int i) const { return i < it.n_tiles ? __ldg(reinterpret_cast<const int2*>(p.tiles) + it.list + i) : make_int2(-1, 0); }
+    __device__ __forceinline__ Walk(const DraftParams& p, const GenericSizes& z, const DraftItem& it, int kvh, uint8_t* stages, int2 first) : p(p), z(z), it(it), kvh(kvh), stages(stages), next(first) {}
     __device__ __forceinline__ Tile take() {
         while (j < it.n_tiles) {
             if (t0 == 0) {
-                const int2 e = __ldg(reinterpret_cast<const int2*>(p.tiles) + it.list + j);
-                chunk = e.x;
-                in_chunk = e.y;
+                chunk = next.x;
+                in_chunk = next.y;
+                next = entry(j + 1);
                 if (chunk < 0 || chunk >= p.max_chunks || in_chunk > p.geo.chunk_size) {
                     if (threadIdx.x == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
                     in_chunk = 0;
@@ -68,27 +70,23 @@ template <typename T> struct Walk {
         d0 += G_TOK;
         return t;
     }
-    // By a whole block.  Parts of chunks whose rows are whole granules by bulk copies of thread 0, which complete on the stage's barrier (true);
+    // By a whole block.  Parts of chunks whose rows are whole granules by bulk copies of warp 0, which complete on the stage's barrier (true);
     // drafted rows of whole granules by asynchronous copies, others by plain ones.  Lines behind the tile's tokens hold anything.
-    __device__ __forceinline__ bool fetch(const Tile& t, int stage, uint32_t bar) const {
+    template <int WARPS> __device__ __forceinline__ bool fetch(const Tile& t, int stage, uint32_t bar) const {
         uint8_t* const sk = stages + stage * z.stage();
         uint8_t* const sv = sk + G_TOK * z.k_bytes;
         const uint32_t to_k = (uint32_t)__cvta_generic_to_shared(sk), to_v = (uint32_t)__cvta_generic_to_shared(sv);
         if (t.chunk >= 0 && p.geo.epg == E) {
-            if (threadIdx.x == 0) {
-                const uint8_t* kt = static_cast<const uint8_t*>(p.pool) + tile_base_elems(p.geo, t.chunk, kvh, 0) * (int)sizeof(T);
-                const uint8_t* vt = kt + p.geo.tile_elems * (int)sizeof(T);
-                ptx::mbar_arrive_expect_tx(bar, t.n * (z.k_bytes + z.v_bytes));
-                auto side = [&](uint32_t to, const uint8_t* from, int row_bytes, int swz) {
-                    if (swz) {
-                        for (int pn = 0; pn < row_bytes / 128; pn++)
-                            ptx::bulk_copy_g2s(to + pn * (G_TOK * 128), from + ((int64_t)pn * p.geo.chunk_size + t.first) * 128, t.n * 128, bar);
-                    } else {
-                        ptx::bulk_copy_g2s(to, from + (int64_t)t.first * row_bytes, t.n * row_bytes, bar);
-                    }
-                };
-                side(to_k, kt, z.k_bytes, p.geo.swz);
-                side(to_v, vt, z.v_bytes, p.geo.v_swz);
+            if (threadIdx.x < 32) {  // a panel or a side to a lane
+                const int lane = threadIdx.x, k_parts = p.geo.swz ? z.k_bytes / 128 : 1, v_parts = p.geo.v_swz ? z.v_bytes / 128 : 1;
+                if (lane == 0) ptx::mbar_arrive_expect_tx(bar, t.n * (z.k_bytes + z.v_bytes));
+                __syncwarp();
+                if (lane < k_parts + v_parts) {
+                    const bool is_v = lane >= k_parts;
+                    const int part = is_v ? lane - k_parts : lane, swz = is_v ? p.geo.v_swz : p.geo.swz, line = swz ? 128 : (is_v ? z.v_bytes : z.k_bytes);
+                    const uint8_t* from = static_cast<const uint8_t*>(p.pool) + (tile_base_elems(p.geo, t.chunk, kvh, 0) + (is_v ? p.geo.tile_elems : 0)) * (int)sizeof(T);
+                    ptx::bulk_copy_g2s((is_v ? to_v : to_k) + part * (G_TOK * 128), from + ((int64_t)part * p.geo.chunk_size + t.first) * line, t.n * line, bar);
+                }
             }
             return true;
         }
@@ -98,14 +96,14 @@ template <typename T> struct Walk {
                 const T* from = static_cast<const T*>(base) + (int64_t)(it.tree + t.first + warp) * node + (int64_t)kvh * head;
                 for (int g = lane; g < row_bytes / 16; g += 32)
 #pragma unroll
-                    for (int i = 0; i < G_TOK / G_WARPS; i++)
-                        if (warp + G_WARPS * i < t.n) cp_async16(to + staged(warp + G_WARPS * i, g, row_bytes, swz), from + i * G_WARPS * node + g * E);
+                    for (int i = 0; i < G_TOK / WARPS; i++)
+                        if (warp + WARPS * i < t.n) cp_async16(to + staged(warp + WARPS * i, g, row_bytes, swz), from + i * WARPS * node + g * E);
             };
             side(to_k, p.k, p.k_node, p.k_head, z.k_bytes, p.geo.swz);
             side(to_v, p.v, p.v_node, p.v_head, z.v_bytes, p.geo.v_swz);
         } else {
             auto side = [&](uint8_t* to, const T* from, int d, int row_bytes, int swz, const Geometry& g, int64_t node) {
-                for (int x = warp; x < t.n; x += G_WARPS)
+                for (int x = warp; x < t.n; x += WARPS)
 #pragma unroll 4
                     for (int e = lane; e < row_bytes / (int)sizeof(T); e += 32) {
                         const T v = e < d ? (t.chunk >= 0 ? from[tile_elem_offset(g, t.first + x, e)] : from[x * node + e]) : from_f32<T>(0.f);
@@ -132,8 +130,8 @@ struct Stages {
     uint32_t bars, used = 0, phases = 0;  // bits: the stage's tile comes by bulk copies, the phase its barrier is in
     long long limit;
     int* status;
-    template <typename T> __device__ __forceinline__ void fetch(const Walk<T>& walk, const Tile& t, int stage) {
-        const bool bulk = walk.fetch(t, stage, bars + 8 * stage);
+    template <int WARPS, typename T> __device__ __forceinline__ void fetch(const Walk<T>& walk, const Tile& t, int stage) {
+        const bool bulk = walk.template fetch<WARPS>(t, stage, bars + 8 * stage);
         used = (used & ~(1u << stage)) | (bulk ? 1u << stage : 0u);
     }
     // The tile of the stage is there, for the whole block.  False: a copy did not come in time; status is recorded
@@ -166,7 +164,7 @@ __device__ __forceinline__ Stages make_stages(const DraftParams& p, uint64_t* ba
     return s;
 }
 // Query rows row, row + step, ... of an item to shared memory as fp32, their loads side by side
-template <typename T, int ROWS> __device__ __forceinline__ void stage_queries(const DraftParams& p, const DraftItem& it, int kvh, float* sq, int q_floats, int n_rows, int row, int step) {
+template <typename T, int ROWS> __device__ __forceinline__ void stage_queries(const DraftParams& p, const DraftItem& it, int kvh, float* sq, int q_floats, int n_rows, int rows, int row, int step) {
     const int lane = threadIdx.x & 31;
     const T* from[ROWS];
 #pragma unroll
@@ -184,7 +182,7 @@ template <typename T, int ROWS> __device__ __forceinline__ void stage_queries(co
         for (int k = 0; k < 4; k++)
 #pragma unroll
             for (int i = 0; i < ROWS; i++)
-                if (e0 + 32 * k < q_floats) sq[(row + step * i) * q_floats + e0 + 32 * k] = x[k][i];
+                if (e0 + 32 * k < q_floats && row + step * i < rows) sq[(row + step * i) * q_floats + e0 + 32 * k] = x[k][i];
     }
 }
 
@@ -204,7 +202,8 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = p.geo.n_heads, group = p.group, H = G * group;
     const int kvh = blockIdx.x % G;
-    const int4 ia = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G)), ib = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 1);
+    const int4 ia = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G)), ib = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 1),
+               ic = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 2);
     const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w, {}};
     if (!draft_item_ok(p, ia, ib, G_WARPS * RW)) {
         if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
@@ -213,7 +212,7 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
     const int n_rows = it.n_nodes * group, row0 = warp * RW;
     const bool busy = row0 < n_rows;
     const int k_gran = whole(dk, E) / E, v_gran = whole(dv, E) / E;  // of a staged row
-    Walk<T> tiles(p, z, it, kvh, stages);
+    Walk<T> tiles(p, z, it, kvh, stages, make_int2(ic.x, ic.y));
     float m[RW], l[RW], o[RW][COLS * 4];
 #pragma unroll
     for (int r = 0; r < RW; r++) {
@@ -227,13 +226,13 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
     Tile now = tiles.take();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (now.n > 0) in.fetch(tiles, now, 0);
+    if (now.n > 0) in.fetch<G_WARPS>(tiles, now, 0);
 #pragma unroll
-    for (int half = 0; half < RW; half += 4) stage_queries<T, 4>(p, it, kvh, sq, z.q_floats, n_rows, row0 + half, 1);
+    for (int half = 0; half < RW; half += 4) stage_queries<T, 4>(p, it, kvh, sq, z.q_floats, n_rows, G_WARPS * RW, row0 + half, 1);
     for (int stage = 0; now.n > 0; stage ^= 1) {
         if (!in.wait(stage)) return;  // nobody reads the tile before this one any more
         const Tile after = tiles.take();
-        if (after.n > 0) in.fetch(tiles, after, stage ^ 1);
+        if (after.n > 0) in.fetch<G_WARPS>(tiles, after, stage ^ 1);
         if (busy) {
             const uint8_t* const sk = stages + stage * stage_bytes;
             const uint8_t* const sv = sk + G_TOK * z.k_bytes;
@@ -368,39 +367,41 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
     }
 }
 
-// The same for at most 16 rows (chains, small trees): the warps share the rows' work instead of the rows.  A warp multiplies a quarter of the
-// key's granules, the quarters meet in shared memory, where every row has its warp for the softmax, and a warp has a quarter of the value's
-// columns, a lane each.  (With a warp's rows its own, few rows leave three warps of every block idle and load one scheduler of the SM: one row
-// of 2000 tokens, 32 fp32 heads of 128, 4 nodes: 62 us.)
+// The same for at most 16 rows (chains, small trees): eight warps share the rows' work instead of the rows.  A warp multiplies an eighth of the
+// key's granules, the parts meet in shared memory, where every row has its warp for the softmax, and a warp has a quarter of the value's
+// columns, a lane each, for half of the tile's tokens.  Bound by the chain of a tile.  (With a warp's rows its own, few rows leave most warps
+// of a block idle and load one scheduler of the SM: one row of 2000 tokens, 32 fp32 heads of 128, 4 nodes: 62 us.)
+constexpr int F_THREADS = 256, F_WARPS = 8;
 template <typename T, int R, int COLS>  // COLS: columns of a lane
-__global__ void __launch_bounds__(G_THREADS) draft_few_kernel(const DraftParams p, const GenericSizes z) {
+__global__ void __launch_bounds__(F_THREADS, 2) draft_few_kernel(const DraftParams p, const GenericSizes z) {
     extern __shared__ __align__(128) uint8_t raw[];
     __shared__ uint64_t bars[G_STAGES];
-    constexpr int E = 16 / sizeof(T), MINE = R / G_WARPS;  // rows of a warp in the softmax
+    constexpr int E = 16 / sizeof(T), MINE = (R + F_WARPS - 1) / F_WARPS;  // rows of a warp in the softmax
     float* const sq = reinterpret_cast<float*>(raw);     // [R][q_floats]
-    float* const ss = sq + R * z.q_floats;               // [4][R][32] quarters of scores
-    float* const sp = ss + G_WARPS * R * G_TOK;          // [R][32] weights
+    float* const ss = sq + R * z.q_floats;               // [8][R][32] parts of scores; at the end [R][128 COLS], one half's output
+    float* const sp = ss + F_WARPS * R * G_TOK;          // [R][32] weights
     float* const sa = sp + R * G_TOK;                    // [R] what the rows' earlier results are scaled by
     float2* const ml = reinterpret_cast<float2*>(sa + R);
-    uint8_t* const stages = raw + whole((int)sizeof(float) * R * (z.q_floats + (G_WARPS + 1) * G_TOK + 3), 128);
+    uint8_t* const stages = raw + whole((int)sizeof(float) * R * (z.q_floats + (F_WARPS + 1) * G_TOK + 3), 128);
     const int dk = p.d_key, dv = p.d_value;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = p.geo.n_heads, group = p.group, H = G * group;
     const int kvh = blockIdx.x % G;
-    const int4 ia = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G)), ib = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 1);
+    const int4* const item = reinterpret_cast<const int4*>(p.items + blockIdx.x / G);
+    const int4 ia = __ldg(item), ib = __ldg(item + 1), ic = __ldg(item + 2);
     const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w, {}};
     if (!draft_item_ok(p, ia, ib, R)) {
         if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
         return;
     }
     const int n_rows = it.n_nodes * group, k_gran = whole(dk, E) / E;
-    Walk<T> tiles(p, z, it, kvh, stages);
+    Walk<T> tiles(p, z, it, kvh, stages, make_int2(ic.x, ic.y));
     Stages in = make_stages(p, bars);
     Tile now = tiles.take();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (now.n > 0) in.fetch(tiles, now, 0);
-    stage_queries<T, MINE>(p, it, kvh, sq, z.q_floats, n_rows, warp, G_WARPS);
+    if (now.n > 0) in.fetch<F_WARPS>(tiles, now, 0);
+    if (warp < R) stage_queries<T, MINE>(p, it, kvh, sq, z.q_floats, n_rows, R, warp, F_WARPS);
     float m[MINE], l[MINE], o[R][COLS];
 #pragma unroll
     for (int i = 0; i < MINE; i++) {
@@ -411,24 +412,31 @@ __global__ void __launch_bounds__(G_THREADS) draft_few_kernel(const DraftParams 
     for (int r = 0; r < R; r++)
 #pragma unroll
         for (int c = 0; c < COLS; c++) o[r][c] = 0.f;
-    const int col0 = warp * 32 * COLS + lane;  // and 32 further
+    const int col0 = (warp & 3) * 32 * COLS + lane;  // and 32 further
+    const int from_token = (warp >> 2) * (G_TOK / 2);
+    // byte of column col0 + 32 c of token t: at[c] + t * v_line + the granule's place in the line, which goes by t & 7
+    const int v_line = p.geo.v_swz ? 128 : z.v_bytes;
+    int at[COLS], place[COLS];
+#pragma unroll
+    for (int c = 0; c < COLS; c++) {
+        const int e = min(col0 + 32 * c, dv - 1), g = e / E;
+        at[c] = G_TOK * z.k_bytes + e % E * (int)sizeof(T) + (p.geo.v_swz ? (g >> 3) * (G_TOK * 128) : g * 16);
+        place[c] = g & 7;
+    }
+    const int swap = p.geo.v_swz ? 7 : 0;
     for (int stage = 0; now.n > 0; stage ^= 1) {
         if (!in.wait(stage)) return;  // nobody reads the tile before this one any more
         const Tile after = tiles.take();
-        if (after.n > 0) in.fetch(tiles, after, stage ^ 1);
+        if (after.n > 0) in.fetch<F_WARPS>(tiles, after, stage ^ 1);
         const uint8_t* const sk = stages + stage * z.stage();
-        const uint8_t* const sv = sk + G_TOK * z.k_bytes;
-        auto value = [&](int t, int c) {
-            const int e = col0 + 32 * c;
-            return e < dv ? to_f32(*reinterpret_cast<const T*>(sv + staged(t, e / E, z.v_bytes, p.geo.v_swz) + e % E * (int)sizeof(T))) : 0.f;
-        };
+        auto value = [&](int t, int c) { return to_f32(*reinterpret_cast<const T*>(sk + at[c] + t * v_line + (swap ? (place[c] ^ (t & 7)) << 4 : 0))); };
         const bool drafted = now.chunk < 0;
         {
             float s[R];
 #pragma unroll
             for (int r = 0; r < R; r++) s[r] = 0.f;
 #pragma unroll 2
-            for (int g = warp; g < k_gran; g += G_WARPS) {
+            for (int g = warp; g < k_gran; g += F_WARPS) {
                 float k[E];
                 Granule<T>::load(reinterpret_cast<const T*>(sk + staged(lane, g, z.k_bytes, p.geo.swz)), k);
 #pragma unroll
@@ -447,18 +455,18 @@ __global__ void __launch_bounds__(G_THREADS) draft_few_kernel(const DraftParams 
         }
         const uint32_t there = now.n == 32 ? 0xffffffffu : (1u << now.n) - 1;
         __syncthreads();
-        {
+        if (warp < R) {
             float s[MINE], high[MINE];
             bool see[MINE];
 #pragma unroll
             for (int i = 0; i < MINE; i++) {
-                const int r = warp + G_WARPS * i;
+                const int r = min(warp + F_WARPS * i, R - 1);
                 uint32_t line = there;
                 if (drafted) line &= __ldg(p.seen + (int64_t)(it.node0 + min(r, n_rows - 1) / group) * p.words + now.first / 32);
                 see[i] = (line >> lane) & 1;
                 float x = 0.f;
 #pragma unroll
-                for (int w = 0; w < G_WARPS; w++) x += ss[(w * R + r) * G_TOK + lane];
+                for (int w = 0; w < F_WARPS; w++) x += ss[(w * R + r) * G_TOK + lane];
                 s[i] = high[i] = see[i] ? x * p.scale_log2 : -INFINITY;
             }
 #pragma unroll
@@ -467,12 +475,14 @@ __global__ void __launch_bounds__(G_THREADS) draft_few_kernel(const DraftParams 
                 for (int i = 0; i < MINE; i++) high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], off));
 #pragma unroll
             for (int i = 0; i < MINE; i++) {
-                const int r = warp + G_WARPS * i;
+                const int r = warp + F_WARPS * i;
                 const float mn = fmaxf(m[i], high[i]), alpha = exp2_approx(m[i] - mn), w = see[i] ? exp2_approx(s[i] - mn) : 0.f;
                 m[i] = mn;
                 l[i] = l[i] * alpha + w;  // this lane's tokens only
-                sp[r * G_TOK + lane] = w;
-                if (lane == 0) sa[r] = alpha;
+                if (r < R) {
+                    sp[r * G_TOK + lane] = w;
+                    if (lane == 0) sa[r] = alpha;
+                }
             }
         }
         __syncthreads();
@@ -484,15 +494,15 @@ __global__ void __launch_bounds__(G_THREADS) draft_few_kernel(const DraftParams 
         }
         if (!drafted && now.n == G_TOK) {
 #pragma unroll 2
-            for (int t = 0; t < G_TOK; t += 4) {
+            for (int t = 0; t < G_TOK / 2; t += 4) {
                 float v[4][COLS];
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int c = 0; c < COLS; c++) v[i][c] = value(t + i, c);
+                    for (int c = 0; c < COLS; c++) v[i][c] = value(from_token + t + i, c);
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    const float4 w = *reinterpret_cast<const float4*>(sp + r * G_TOK + t);
+                    const float4 w = *reinterpret_cast<const float4*>(sp + r * G_TOK + from_token + t);
 #pragma unroll
                     for (int c = 0; c < COLS; c++) {
                         o[r][c] = fmaf(w.x, v[0][c], o[r][c]);
@@ -505,17 +515,17 @@ __global__ void __launch_bounds__(G_THREADS) draft_few_kernel(const DraftParams 
         } else {
             // values that a row does not see may be infinite: they are left out, not multiplied by zero
             uint32_t line[R];
-            int node = it.node0, head = 0;
+            int node = it.node0, in_group = 0;
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 line[r] = drafted && r < n_rows ? there & __ldg(p.seen + (int64_t)node * p.words + now.first / 32) : there;
-                if (++head == group) {
-                    head = 0;
+                if (++in_group == group) {
+                    in_group = 0;
                     node++;
                 }
             }
 #pragma unroll 1
-            for (int t = 0; t < now.n; t++) {
+            for (int t = from_token; t < min(now.n, from_token + G_TOK / 2); t++) {
                 float v[COLS];
 #pragma unroll
                 for (int c = 0; c < COLS; c++) v[c] = value(t, c);
@@ -529,31 +539,41 @@ __global__ void __launch_bounds__(G_THREADS) draft_few_kernel(const DraftParams 
         }
         now = after;
     }
+    if (warp < R) {
 #pragma unroll
-    for (int i = 0; i < MINE; i++) {
-        const float sum = warp_sum(l[i]);
-        if (lane == 0) ml[warp + G_WARPS * i] = make_float2(m[i], sum);
+        for (int i = 0; i < MINE; i++) {
+            const float sum = warp_sum(l[i]);
+            if (lane == 0 && warp + F_WARPS * i < R) ml[warp + F_WARPS * i] = make_float2(m[i], sum);
+        }
+    }
+    // the halves meet; the parts of scores have been read long ago
+    if (warp >= 4) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int c = 0; c < COLS; c++) ss[r * 128 * COLS + col0 + 32 * c] = o[r][c];
     }
     __syncthreads();
+    if (warp >= 4) return;
     int at_node = 0, in_group = 0;
 #pragma unroll
     for (int r = 0; r < R; r++) {
         if (r >= n_rows) break;
         const int head = kvh * group + in_group;
         const float2 own = ml[r];
-        if (it.slot >= 0) {
-            const int64_t at = (int64_t)(it.slot + at_node) * H + head;
-            if (tid == 0) p.part_ml[at] = own;
+        const float M = p.sink && it.slot < 0 ? fmaxf(own.x, 0.f) : own.x;
+        const float w = exp2_approx(own.x - M), total = own.y * w + (p.sink ? exp2_approx(-M) : 0.f), scale = total == 0.f ? 0.f : w / total;
+        const int64_t row = (int64_t)((it.slot >= 0 ? it.slot : it.node0) + at_node) * H + head;
+        if (it.slot >= 0 && tid == 0) p.part_ml[row] = own;
 #pragma unroll
-            for (int c = 0; c < COLS; c++)
-                if (col0 + 32 * c < p.part_width) p.part_o[at * p.part_width + col0 + 32 * c] = o[r][c];
-        } else {
-            const float M = p.sink ? fmaxf(own.x, 0.f) : own.x;
-            const float w = exp2_approx(own.x - M), total = own.y * w + (p.sink ? exp2_approx(-M) : 0.f), scale = total == 0.f ? 0.f : w / total;
-            T* out = static_cast<T*>(p.out) + ((int64_t)(it.node0 + at_node) * H + head) * dv;
-#pragma unroll
-            for (int c = 0; c < COLS; c++)
-                if (col0 + 32 * c < dv) out[col0 + 32 * c] = from_f32<T>(o[r][c] * scale);
+        for (int c = 0; c < COLS; c++) {
+            const int e = col0 + 32 * c;
+            const float x = o[r][c] + ss[r * 128 * COLS + e];
+            if (it.slot >= 0) {
+                if (e < p.part_width) p.part_o[row * p.part_width + e] = x;
+            } else if (e < dv) {
+                static_cast<T*>(p.out)[row * dv + e] = from_f32<T>(x * scale);
+            }
         }
         if (++in_group == group) {
             in_group = 0;
@@ -565,15 +585,15 @@ __global__ void __launch_bounds__(G_THREADS) draft_few_kernel(const DraftParams 
 template <typename T>
 cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t stream) {
     const GenericSizes z = generic_sizes(p.d_key, p.d_value, sizeof(T));
-    auto go = [&](auto* k, size_t floats) {
+    auto go = [&](auto* k, int threads, size_t floats) {
         const size_t smem = whole((int)(sizeof(float) * floats), 128) + (size_t)G_STAGES * z.stage();
         cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         if (e != cudaSuccess) return e;
-        return launch_kernel(k, dim3((unsigned)p.n_items * p.geo.n_heads), G_THREADS, smem, 1, p.dependent & DEPENDENT_ATTENTION, stream, p, z);
+        return launch_kernel(k, dim3((unsigned)p.n_items * p.geo.n_heads), threads, smem, 1, p.dependent & DEPENDENT_ATTENTION, stream, p, z);
     };
-    auto few = [&](auto* k, int r) { return go(k, (size_t)r * (z.q_floats + (G_WARPS + 1) * G_TOK + 3)); };
-    auto many = [&](auto* k, int rw) { return go(k, (size_t)G_WARPS * rw * (z.q_floats + G_TOK)); };
+    auto few = [&](auto* k, int r) { return go(k, F_THREADS, (size_t)r * (z.q_floats + (F_WARPS + 1) * G_TOK + 3)); };
+    auto many = [&](auto* k, int rw) { return go(k, G_THREADS, (size_t)G_WARPS * rw * (z.q_floats + G_TOK)); };
     if (p.d_value <= 128) {
         if (block_rows <= 4) return few(&draft_few_kernel<T, 4, 1>, 4);
         if (block_rows <= 8) return few(&draft_few_kernel<T, 8, 1>, 8);
@@ -721,7 +741,7 @@ __global__ void __launch_bounds__(32) accept_draft_kernel(const AcceptParams p) 
 
 int draft_generic_ctas(int block_rows, int dk, int dv, int esize) {
     const GenericSizes z = generic_sizes(dk, dv, esize);
-    const int rows = sizeof(float) * block_rows * (z.q_floats + (block_rows <= 16 ? (G_WARPS + 1) * G_TOK + 3 : G_TOK));
+    const int rows = sizeof(float) * block_rows * (z.q_floats + (block_rows <= 16 ? (F_WARPS + 1) * G_TOK + 3 : G_TOK));
     return B200_SMS * std::max(1, std::min(4, 232448 / (rows + G_STAGES * z.stage() + 1024 + 128)));
 }
 
