@@ -16,7 +16,7 @@
 namespace ca {
 namespace {
 
-constexpr int G_THREADS = 128, G_WARPS = 4, G_TOK = 32, G_STAGES = 2;
+constexpr int G_THREADS = 256, G_WARPS = 8, G_TOK = 32, G_STAGES = 2;
 constexpr float G_NEG_BIG = -1.0e30f;
 
 __host__ __device__ constexpr int whole(int x, int unit) { return (x + unit - 1) / unit * unit; }
@@ -72,7 +72,7 @@ template <typename T> struct Walk {
     }
     // By a whole block.  Parts of chunks whose rows are whole granules by bulk copies of warp 0, which complete on the stage's barrier (true);
     // drafted rows of whole granules by asynchronous copies, others by plain ones.  Lines behind the tile's tokens hold anything.
-    template <int WARPS> __device__ __forceinline__ bool fetch(const Tile& t, int stage, uint32_t bar) const {
+    __device__ __forceinline__ bool fetch(const Tile& t, int stage, uint32_t bar) const {
         uint8_t* const sk = stages + stage * z.stage();
         uint8_t* const sv = sk + G_TOK * z.k_bytes;
         const uint32_t to_k = (uint32_t)__cvta_generic_to_shared(sk), to_v = (uint32_t)__cvta_generic_to_shared(sv);
@@ -96,14 +96,14 @@ template <typename T> struct Walk {
                 const T* from = static_cast<const T*>(base) + (int64_t)(it.tree + t.first + warp) * node + (int64_t)kvh * head;
                 for (int g = lane; g < row_bytes / 16; g += 32)
 #pragma unroll
-                    for (int i = 0; i < G_TOK / WARPS; i++)
-                        if (warp + WARPS * i < t.n) cp_async16(to + staged(warp + WARPS * i, g, row_bytes, swz), from + i * WARPS * node + g * E);
+                    for (int i = 0; i < G_TOK / G_WARPS; i++)
+                        if (warp + G_WARPS * i < t.n) cp_async16(to + staged(warp + G_WARPS * i, g, row_bytes, swz), from + i * G_WARPS * node + g * E);
             };
             side(to_k, p.k, p.k_node, p.k_head, z.k_bytes, p.geo.swz);
             side(to_v, p.v, p.v_node, p.v_head, z.v_bytes, p.geo.v_swz);
         } else {
             auto side = [&](uint8_t* to, const T* from, int d, int row_bytes, int swz, const Geometry& g, int64_t node) {
-                for (int x = warp; x < t.n; x += WARPS)
+                for (int x = warp; x < t.n; x += G_WARPS)
 #pragma unroll 4
                     for (int e = lane; e < row_bytes / (int)sizeof(T); e += 32) {
                         const T v = e < d ? (t.chunk >= 0 ? from[tile_elem_offset(g, t.first + x, e)] : from[x * node + e]) : from_f32<T>(0.f);
@@ -130,8 +130,8 @@ struct Stages {
     uint32_t bars, used = 0, phases = 0;  // bits: the stage's tile comes by bulk copies, the phase its barrier is in
     long long limit;
     int* status;
-    template <int WARPS, typename T> __device__ __forceinline__ void fetch(const Walk<T>& walk, const Tile& t, int stage) {
-        const bool bulk = walk.template fetch<WARPS>(t, stage, bars + 8 * stage);
+    template <typename T> __device__ __forceinline__ void fetch(const Walk<T>& walk, const Tile& t, int stage) {
+        const bool bulk = walk.fetch(t, stage, bars + 8 * stage);
         used = (used & ~(1u << stage)) | (bulk ? 1u << stage : 0u);
     }
     // The tile of the stage is there, for the whole block.  False: a copy did not come in time; status is recorded
@@ -186,17 +186,17 @@ template <typename T, int ROWS> __device__ __forceinline__ void stage_queries(co
     }
 }
 
-// An item for one key/value head.  Four warps with RW query rows each (row r: query head r % group of node r / group); the keys go by in tiles of
+// An item for one key/value head.  Eight warps with RW query rows each (row r: query head r % group of node r / group); the keys go by in tiles of
 // 32 tokens, staged as they are, the next one on its way.  Scores: a lane has a token, and multiplies its key with the warp's rows (read by all
 // lanes at once).  Softmax: over the lanes, the rows' steps side by side.  Output: a lane has the columns 4 lane .. 4 lane + 3 of each 128,
 // weights come from shared memory.  For 17 rows and more; bound by fp32 products and the reads that feed them.
 template <typename T, int RW, int COLS>  // COLS: groups of 128 value columns
-__global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftParams p, const GenericSizes z) {
+__global__ void __launch_bounds__(G_THREADS, 2) draft_generic_kernel(const DraftParams p, const GenericSizes z) {
     extern __shared__ __align__(128) uint8_t raw[];
     __shared__ uint64_t bars[G_STAGES];
     constexpr int E = 16 / sizeof(T);
-    float* const sq = reinterpret_cast<float*>(raw);     // [4 RW][q_floats]
-    float* const sp = sq + G_WARPS * RW * z.q_floats;    // [4 RW][32] weights
+    float* const sq = reinterpret_cast<float*>(raw);     // [8 RW][q_floats]
+    float* const sp = sq + G_WARPS * RW * z.q_floats;    // [8 RW][32] weights
     uint8_t* const stages = raw + whole((int)sizeof(float) * G_WARPS * RW * (z.q_floats + G_TOK), 128);
     const int dk = p.d_key, dv = p.d_value, stage_bytes = z.stage();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -226,13 +226,13 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
     Tile now = tiles.take();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (now.n > 0) in.fetch<G_WARPS>(tiles, now, 0);
+    if (now.n > 0) in.fetch(tiles, now, 0);
 #pragma unroll
     for (int half = 0; half < RW; half += 4) stage_queries<T, 4>(p, it, kvh, sq, z.q_floats, n_rows, G_WARPS * RW, row0 + half, 1);
     for (int stage = 0; now.n > 0; stage ^= 1) {
         if (!in.wait(stage)) return;  // nobody reads the tile before this one any more
         const Tile after = tiles.take();
-        if (after.n > 0) in.fetch<G_WARPS>(tiles, after, stage ^ 1);
+        if (after.n > 0) in.fetch(tiles, after, stage ^ 1);
         if (busy) {
             const uint8_t* const sk = stages + stage * stage_bytes;
             const uint8_t* const sv = sk + G_TOK * z.k_bytes;
@@ -371,18 +371,17 @@ __global__ void __launch_bounds__(G_THREADS) draft_generic_kernel(const DraftPar
 // key's granules, the parts meet in shared memory, where every row has its warp for the softmax, and a warp has a quarter of the value's
 // columns, a lane each, for half of the tile's tokens.  Bound by the chain of a tile.  (With a warp's rows its own, few rows leave most warps
 // of a block idle and load one scheduler of the SM: one row of 2000 tokens, 32 fp32 heads of 128, 4 nodes: 62 us.)
-constexpr int F_THREADS = 256, F_WARPS = 8;
 template <typename T, int R, int COLS>  // COLS: columns of a lane
-__global__ void __launch_bounds__(F_THREADS, 2) draft_few_kernel(const DraftParams p, const GenericSizes z) {
+__global__ void __launch_bounds__(G_THREADS, 2) draft_few_kernel(const DraftParams p, const GenericSizes z) {
     extern __shared__ __align__(128) uint8_t raw[];
     __shared__ uint64_t bars[G_STAGES];
-    constexpr int E = 16 / sizeof(T), MINE = (R + F_WARPS - 1) / F_WARPS;  // rows of a warp in the softmax
+    constexpr int E = 16 / sizeof(T), MINE = (R + G_WARPS - 1) / G_WARPS;  // rows of a warp in the softmax
     float* const sq = reinterpret_cast<float*>(raw);     // [R][q_floats]
     float* const ss = sq + R * z.q_floats;               // [8][R][32] parts of scores; at the end [R][128 COLS], one half's output
-    float* const sp = ss + F_WARPS * R * G_TOK;          // [R][32] weights
+    float* const sp = ss + G_WARPS * R * G_TOK;          // [R][32] weights
     float* const sa = sp + R * G_TOK;                    // [R] what the rows' earlier results are scaled by
     float2* const ml = reinterpret_cast<float2*>(sa + R);
-    uint8_t* const stages = raw + whole((int)sizeof(float) * R * (z.q_floats + (F_WARPS + 1) * G_TOK + 3), 128);
+    uint8_t* const stages = raw + whole((int)sizeof(float) * R * (z.q_floats + (G_WARPS + 1) * G_TOK + 3), 128);
     const int dk = p.d_key, dv = p.d_value;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = p.geo.n_heads, group = p.group, H = G * group;
@@ -400,8 +399,8 @@ __global__ void __launch_bounds__(F_THREADS, 2) draft_few_kernel(const DraftPara
     Tile now = tiles.take();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (now.n > 0) in.fetch<F_WARPS>(tiles, now, 0);
-    if (warp < R) stage_queries<T, MINE>(p, it, kvh, sq, z.q_floats, n_rows, R, warp, F_WARPS);
+    if (now.n > 0) in.fetch(tiles, now, 0);
+    if (warp < R) stage_queries<T, MINE>(p, it, kvh, sq, z.q_floats, n_rows, R, warp, G_WARPS);
     float m[MINE], l[MINE], o[R][COLS];
 #pragma unroll
     for (int i = 0; i < MINE; i++) {
@@ -427,7 +426,7 @@ __global__ void __launch_bounds__(F_THREADS, 2) draft_few_kernel(const DraftPara
     for (int stage = 0; now.n > 0; stage ^= 1) {
         if (!in.wait(stage)) return;  // nobody reads the tile before this one any more
         const Tile after = tiles.take();
-        if (after.n > 0) in.fetch<F_WARPS>(tiles, after, stage ^ 1);
+        if (after.n > 0) in.fetch(tiles, after, stage ^ 1);
         const uint8_t* const sk = stages + stage * z.stage();
         auto value = [&](int t, int c) { return to_f32(*reinterpret_cast<const T*>(sk + at[c] + t * v_line + (swap ? (place[c] ^ (t & 7)) << 4 : 0))); };
         const bool drafted = now.chunk < 0;
@@ -436,7 +435,7 @@ __global__ void __launch_bounds__(F_THREADS, 2) draft_few_kernel(const DraftPara
 #pragma unroll
             for (int r = 0; r < R; r++) s[r] = 0.f;
 #pragma unroll 2
-            for (int g = warp; g < k_gran; g += F_WARPS) {
+            for (int g = warp; g < k_gran; g += G_WARPS) {
                 float k[E];
                 Granule<T>::load(reinterpret_cast<const T*>(sk + staged(lane, g, z.k_bytes, p.geo.swz)), k);
 #pragma unroll
@@ -460,13 +459,13 @@ __global__ void __launch_bounds__(F_THREADS, 2) draft_few_kernel(const DraftPara
             bool see[MINE];
 #pragma unroll
             for (int i = 0; i < MINE; i++) {
-                const int r = min(warp + F_WARPS * i, R - 1);
+                const int r = min(warp + G_WARPS * i, R - 1);
                 uint32_t line = there;
                 if (drafted) line &= __ldg(p.seen + (int64_t)(it.node0 + min(r, n_rows - 1) / group) * p.words + now.first / 32);
                 see[i] = (line >> lane) & 1;
                 float x = 0.f;
 #pragma unroll
-                for (int w = 0; w < F_WARPS; w++) x += ss[(w * R + r) * G_TOK + lane];
+                for (int w = 0; w < G_WARPS; w++) x += ss[(w * R + r) * G_TOK + lane];
                 s[i] = high[i] = see[i] ? x * p.scale_log2 : -INFINITY;
             }
 #pragma unroll
@@ -475,7 +474,7 @@ __global__ void __launch_bounds__(F_THREADS, 2) draft_few_kernel(const DraftPara
                 for (int i = 0; i < MINE; i++) high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], off));
 #pragma unroll
             for (int i = 0; i < MINE; i++) {
-                const int r = warp + F_WARPS * i;
+                const int r = warp + G_WARPS * i;
                 const float mn = fmaxf(m[i], high[i]), alpha = exp2_approx(m[i] - mn), w = see[i] ? exp2_approx(s[i] - mn) : 0.f;
                 m[i] = mn;
                 l[i] = l[i] * alpha + w;  // this lane's tokens only
@@ -543,7 +542,7 @@ __global__ void __launch_bounds__(F_THREADS, 2) draft_few_kernel(const DraftPara
 #pragma unroll
         for (int i = 0; i < MINE; i++) {
             const float sum = warp_sum(l[i]);
-            if (lane == 0 && warp + F_WARPS * i < R) ml[warp + F_WARPS * i] = make_float2(m[i], sum);
+            if (lane == 0 && warp + G_WARPS * i < R) ml[warp + G_WARPS * i] = make_float2(m[i], sum);
         }
     }
     // the halves meet; the parts of scores have been read long ago
@@ -592,22 +591,22 @@ cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t st
         if (e != cudaSuccess) return e;
         return launch_kernel(k, dim3((unsigned)p.n_items * p.geo.n_heads), threads, smem, 1, p.dependent & DEPENDENT_ATTENTION, stream, p, z);
     };
-    auto few = [&](auto* k, int r) { return go(k, F_THREADS, (size_t)r * (z.q_floats + (F_WARPS + 1) * G_TOK + 3)); };
+    auto few = [&](auto* k, int r) { return go(k, G_THREADS, (size_t)r * (z.q_floats + (G_WARPS + 1) * G_TOK + 3)); };
     auto many = [&](auto* k, int rw) { return go(k, G_THREADS, (size_t)G_WARPS * rw * (z.q_floats + G_TOK)); };
     if (p.d_value <= 128) {
         if (block_rows <= 4) return few(&draft_few_kernel<T, 4, 1>, 4);
         if (block_rows <= 8) return few(&draft_few_kernel<T, 8, 1>, 8);
         if (block_rows <= 12) return few(&draft_few_kernel<T, 12, 1>, 12);
         if (block_rows <= 16) return few(&draft_few_kernel<T, 16, 1>, 16);
-        if (block_rows <= 32) return many(&draft_generic_kernel<T, 8, 1>, 8);
-        return many(&draft_generic_kernel<T, 16, 1>, 16);
+        if (block_rows <= 32) return many(&draft_generic_kernel<T, 4, 1>, 4);
+        return many(&draft_generic_kernel<T, 8, 1>, 8);
     }
     if (block_rows <= 4) return few(&draft_few_kernel<T, 4, 2>, 4);
     if (block_rows <= 8) return few(&draft_few_kernel<T, 8, 2>, 8);
     if (block_rows <= 12) return few(&draft_few_kernel<T, 12, 2>, 12);
     if (block_rows <= 16) return few(&draft_few_kernel<T, 16, 2>, 16);
-    if (block_rows <= 32) return many(&draft_generic_kernel<T, 8, 2>, 8);
-    return many(&draft_generic_kernel<T, 16, 2>, 16);
+    if (block_rows <= 32) return many(&draft_generic_kernel<T, 4, 2>, 4);
+    return many(&draft_generic_kernel<T, 8, 2>, 8);
 }
 
 // ---- combination: a warp for every (node, query head) that several items serve ---------------------------------------------------
@@ -741,8 +740,8 @@ __global__ void __launch_bounds__(32) accept_draft_kernel(const AcceptParams p) 
 
 int draft_generic_ctas(int block_rows, int dk, int dv, int esize) {
     const GenericSizes z = generic_sizes(dk, dv, esize);
-    const int rows = sizeof(float) * block_rows * (z.q_floats + (block_rows <= 16 ? (F_WARPS + 1) * G_TOK + 3 : G_TOK));
-    return B200_SMS * std::max(1, std::min(4, 232448 / (rows + G_STAGES * z.stage() + 1024 + 128)));
+    const int rows = sizeof(float) * block_rows * (z.q_floats + (block_rows <= 16 ? (G_WARPS + 1) * G_TOK + 3 : G_TOK));
+    return B200_SMS * std::max(1, std::min(2, 232448 / (rows + G_STAGES * z.stage() + 1024 + 128)));
 }
 
 cudaError_t launch_draft_generic(const DraftParams& p, int block_rows, int dtype, cudaStream_t stream) {
