@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "ca_draft.h"
+#include "ca_draft_row.cuh"
 #include "ca_kernels.h"
 #include "ca_launch.cuh"
 #include "ca_ptx.cuh"
@@ -581,6 +582,203 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_few_kernel(const DraftPara
     }
 }
 
+// fp32 with 17 rows and more, heads of 64 or 128: both products on the tensor cores (mma.sync, tf32), every operand as the sum of two tf32
+// numbers of 11 bits and three products of the four, which leaves out 2^-22 of a product: fp32 products on the CUDA cores ran at 9 TFLOP/s.
+// A block has 64 (32) rows; its warps are 4 (2) tiles of 16 rows times 2 (4) shares of every tile's 32 tokens, which meet at the end.
+// S = Q K^T: m16n8k8, A = queries, B = keys.  O += P V: the weights stay where the scores were, if an MMA's k index 2 j + i is token 2 j + i for
+// column j + 4 i: the values' rows are read in that order.
+struct Tf32Pair { uint32_t hi, lo; };
+__device__ __forceinline__ Tf32Pair split_tf32(float x) {
+    Tf32Pair r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.hi) : "f"(x));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.lo) : "f"(x - __uint_as_float(r.hi)));
+    return r;
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_pairs(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], Tf32Pair b0, Tf32Pair b1) {
+    mma_tf32(d, al, b0.hi, b1.hi);
+    mma_tf32(d, ah, b0.lo, b1.lo);
+    mma_tf32(d, ah, b0.hi, b1.hi);
+}
+
+template <int D, int MT>  // head size; tiles of 16 rows
+__global__ void __launch_bounds__(G_THREADS, 2) draft_tf32_kernel(const __grid_constant__ DraftParams p, const GenericSizes z) {
+    extern __shared__ __align__(128) uint8_t raw[];
+    __shared__ uint64_t bars[G_STAGES];
+    constexpr int SHARES = G_WARPS / MT, NT = G_TOK / SHARES / 8, ROWS = 16 * MT, QP = D + 4, OP = D + 4;
+    float* const sq = reinterpret_cast<float*>(raw);     // [ROWS][QP]
+    uint8_t* const stages = raw + whole((int)sizeof(float) * ROWS * QP, 128);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, oct = lane >> 2;
+    const int G = p.geo.n_heads, group = p.group, H = G * group;
+    const int kvh = blockIdx.x % G;
+    const int4* const item = reinterpret_cast<const int4*>(p.items + blockIdx.x / G);
+    const int4 ia = __ldg(item), ib = __ldg(item + 1), ic = __ldg(item + 2);
+    const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w, {}};
+    if (!draft_item_ok(p, ia, ib, ROWS)) {
+        if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
+        return;
+    }
+    const int n_rows = it.n_nodes * group, row0 = (warp % MT) * 16, tok0 = (warp / MT) * (G_TOK / SHARES);
+    const bool busy = row0 < n_rows;
+    Walk<float> tiles(p, z, it, kvh, stages, make_int2(ic.x, ic.y));
+    Stages in = make_stages(p, bars);
+    Tile now = tiles.take();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (now.n > 0) in.fetch(tiles, now, 0);
+#pragma unroll
+    for (int half = 0; half < ROWS / G_WARPS; half += 4) stage_queries<float, 4>(p, it, kvh, sq, QP, n_rows, ROWS, warp * (ROWS / G_WARPS) + half, 1);
+    float o[D / 8][4], m[2] = {G_NEG_BIG, G_NEG_BIG}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < D / 8; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[i][k] = 0.f;
+    const uint32_t* line[2];  // of rows oct and oct + 8
+#pragma unroll
+    for (int h = 0; h < 2; h++) line[h] = p.seen + (int64_t)(it.node0 + min(row0 + oct + 8 * h, n_rows - 1) / group) * p.words;
+    for (int stage = 0; now.n > 0; stage ^= 1) {
+        if (!in.wait(stage)) return;  // nobody reads the tile before this one any more
+        const Tile after = tiles.take();
+        if (after.n > 0) in.fetch(tiles, after, stage ^ 1);
+        if (busy && tok0 < now.n) {
+            const uint8_t* const sk = stages + stage * z.stage();
+            const uint8_t* const sv = sk + G_TOK * z.k_bytes;
+            uint32_t see[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                see[h] = now.n == 32 ? 0xffffffffu : (1u << now.n) - 1;
+                if (now.chunk < 0) see[h] &= __ldg(line[h] + now.first / 32);
+            }
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) s[n][k] = 0.f;
+#pragma unroll 2
+            for (int ks = 0; ks < D / 8; ks++) {
+                uint32_t ah[4], al[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const Tf32Pair a = split_tf32(sq[(row0 + oct + 8 * (k & 1)) * QP + 8 * ks + quad + 4 * (k >> 1)]);
+                    ah[k] = a.hi;
+                    al[k] = a.lo;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const int t = tok0 + 8 * n + oct;
+                    const float b0 = *reinterpret_cast<const float*>(sk + staged(t, 2 * ks, 0, 7) + 4 * quad), b1 = *reinterpret_cast<const float*>(sk + staged(t, 2 * ks + 1, 0, 7) + 4 * quad);
+                    mma_pairs(s[n], ah, al, split_tf32(b0), split_tf32(b1));
+                }
+            }
+            float high[2] = {G_NEG_BIG, G_NEG_BIG};
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    s[n][k] = (see[k >> 1] >> (tok0 + 8 * n + 2 * quad + (k & 1))) & 1 ? s[n][k] * p.scale_log2 : -INFINITY;
+                    high[k >> 1] = fmaxf(high[k >> 1], s[n][k]);
+                }
+            float alpha[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                high[h] = fmaxf(high[h], __shfl_xor_sync(0xffffffffu, high[h], 1));
+                high[h] = fmaxf(high[h], __shfl_xor_sync(0xffffffffu, high[h], 2));
+                const float mn = fmaxf(m[h], high[h]);
+                alpha[h] = exp2_approx(m[h] - mn);
+                m[h] = mn;
+                l[h] *= alpha[h];
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    s[n][k] = exp2_approx(s[n][k] - m[k >> 1]);
+                    l[k >> 1] += s[n][k];  // this lane's columns only: summed over the quad at the end
+                }
+            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) o[i][k] *= alpha[k >> 1];
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                uint32_t ah[4], al[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {  // A: row oct | oct + 8 of columns quad, then of quad + 4
+                    const Tf32Pair a = split_tf32(s[n][2 * (k & 1) + (k >> 1)]);
+                    ah[k] = a.hi;
+                    al[k] = a.lo;
+                }
+                // values behind the tile's tokens are anything: zero
+                const int t = tok0 + 8 * n + 2 * quad;
+                const bool on0 = t < now.n, on1 = t + 1 < now.n;
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) {
+                    const int c = 8 * i + oct;
+                    const float b0 = *reinterpret_cast<const float*>(sv + staged(t, c >> 2, 0, 7) + 4 * (c & 3)), b1 = *reinterpret_cast<const float*>(sv + staged(t + 1, c >> 2, 0, 7) + 4 * (c & 3));
+                    mma_pairs(o[i], ah, al, split_tf32(on0 ? b0 : 0.f), split_tf32(on1 ? b1 : 0.f));
+                }
+            }
+        }
+        now = after;
+    }
+    // ---- the shares of a row meet
+    __syncthreads();
+    float* const so = reinterpret_cast<float*>(raw);                     // [8 warps][16][OP]
+    float2* const ml = reinterpret_cast<float2*>(so + G_WARPS * 16 * OP);  // [8 warps][16]
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        const int r = warp * 16 + oct + 8 * h;
+        if (quad == 0) ml[r] = make_float2(m[h], l[h]);
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) *reinterpret_cast<float2*>(so + r * OP + 8 * i + 2 * quad) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+    }
+    __syncthreads();
+    for (int r = warp; r < n_rows; r += G_WARPS) {
+        const int at_node = r / group, head = kvh * group + r - at_node * group, from = (r / 16) * 16 + r % 16;
+        float M = p.sink && it.slot < 0 ? 0.f : G_NEG_BIG, w[SHARES], total = 0.f;
+#pragma unroll
+        for (int k = 0; k < SHARES; k++) M = fmaxf(M, ml[from + k * 16 * MT].x);
+#pragma unroll
+        for (int k = 0; k < SHARES; k++) {
+            const float2 part = ml[from + k * 16 * MT];
+            w[k] = exp2_approx(part.x - M);
+            total = fmaf(part.y, w[k], total);
+        }
+        float x[D / 32], bad = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) {
+            x[c] = 0.f;
+#pragma unroll
+            for (int k = 0; k < SHARES; k++) x[c] = fmaf(w[k], so[(from + k * 16 * MT) * OP + 32 * c + lane], x[c]);
+            bad = fmaf(0.f, x[c], bad);
+        }
+        if (__any_sync(0xffffffffu, !(bad + 0.f * total == 0.f))) {
+            // something infinite, perhaps where the row does not look: once more, a key at a time
+            row_again<float>(p, it, kvh, r, lane);
+            continue;
+        }
+        const int64_t row = (int64_t)((it.slot >= 0 ? it.slot : it.node0) + at_node) * H + head;
+        if (it.slot >= 0) {
+            if (lane == 0) p.part_ml[row] = make_float2(M, total);
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) p.part_o[row * p.part_width + 32 * c + lane] = x[c];
+        } else {
+            if (p.sink) total += exp2_approx(-M);
+            const float scale = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) static_cast<float*>(p.out)[row * D + 32 * c + lane] = x[c] * scale;
+        }
+    }
+}
+
 template <typename T>
 cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t stream) {
     const GenericSizes z = generic_sizes(p.d_key, p.d_value, sizeof(T));
@@ -593,6 +791,13 @@ cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t st
     };
     auto few = [&](auto* k, int r) { return go(k, G_THREADS, (size_t)r * (z.q_floats + (G_WARPS + 1) * G_TOK + 3)); };
     auto many = [&](auto* k, int rw) { return go(k, G_THREADS, (size_t)G_WARPS * rw * (z.q_floats + G_TOK)); };
+    if constexpr (sizeof(T) == 4) {
+        if (block_rows > 16 && p.d_key == p.d_value && (p.d_key == 64 || p.d_key == 128) && p.geo.swz && p.geo.v_swz) {
+            auto tf32 = [&](auto* k, int rows, int d) { return go(k, G_THREADS, std::max((size_t)rows * (d + 4), (size_t)G_WARPS * 16 * (d + 6) - G_STAGES * z.stage() / 4)); };
+            if (p.d_key == 64) return block_rows <= 32 ? tf32(&draft_tf32_kernel<64, 2>, 32, 64) : tf32(&draft_tf32_kernel<64, 4>, 64, 64);
+            return block_rows <= 32 ? tf32(&draft_tf32_kernel<128, 2>, 32, 128) : tf32(&draft_tf32_kernel<128, 4>, 64, 128);
+        }
+    }
     if (p.d_value <= 128) {
         if (block_rows <= 4) return few(&draft_few_kernel<T, 4, 1>, 4);
         if (block_rows <= 8) return few(&draft_few_kernel<T, 8, 1>, 8);

@@ -24,6 +24,7 @@
 #include <atomic>
 
 #include "ca_draft.h"
+#include "ca_draft_row.cuh"
 #include "ca_kernels.h"
 #include "ca_launch.cuh"
 #include "ca_ptx.cuh"
@@ -85,55 +86,6 @@ template <int DK, int DV> struct Sizes {
     static constexpr int WORK = OUT + A_ROWS * OUT_PITCH, CLC = WORK + 2 * (int)sizeof(Work), BARS = CLC + 16;
     static constexpr int SMEM = BARS + A_NUM_BARS * 8 + 8;
 };
-
-// One row of a piece once more, by a warp: lane e has the elements e, e + 32, ...
-template <typename T>
-__device__ __noinline__ void row_again(const DraftParams& p, const Work& w, int r, int lane) {
-    const int G = p.geo.n_heads, group = p.group, H = G * group, dk = p.d_key, dv = p.d_value;
-    const int node = w.node0 + r / group, head = w.kvh * group + r % group;
-    const T* q = static_cast<const T*>(p.q) + (int64_t)node * p.q_node + (int64_t)head * p.q_head;
-    float qe[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = A_NEG_BIG, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) qe[i] = lane + 32 * i < dk ? to_f32(q[lane + 32 * i]) : 0.f;
-    const Geometry vs = tile_side(p.geo, 1);
-    auto take = [&](auto key, auto value) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 32 * i < dk) s = fmaf(qe[i], key(lane + 32 * i), s);
-        s = warp_sum(s) * p.scale_log2;
-        const float mn = fmaxf(m, s), alpha = exp2f(m - mn), x = exp2f(s - mn);
-        m = mn;
-        l = l * alpha + x;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 32 * i < dv) o[i] = o[i] * alpha + x * value(lane + 32 * i);
-    };
-    for (int j = 0; j < w.n_context; j++) {
-        const int chunk = p.tiles[2 * (w.list + j)], n = min(p.tiles[2 * (w.list + j) + 1], A_TOK);
-        if (chunk < 0 || chunk >= p.max_chunks) continue;
-        const T* kt = static_cast<const T*>(p.pool) + tile_base_elems(p.geo, chunk, w.kvh, 0);
-        const T* vt = kt + p.geo.tile_elems;
-        for (int t = 0; t < n; t++)
-            take([&](int e) { return to_f32(kt[tile_elem_offset(p.geo, t, e)]); }, [&](int e) { return to_f32(vt[tile_elem_offset(vs, t, e)]); });
-    }
-    for (int t = 0; t < w.n_drafted; t++) {
-        if (!((p.seen[(int64_t)node * p.words + t / 32] >> (t & 31)) & 1)) continue;
-        const T* k = static_cast<const T*>(p.k) + (int64_t)(w.tree + t) * p.k_node + (int64_t)w.kvh * p.k_head;
-        const T* v = static_cast<const T*>(p.v) + (int64_t)(w.tree + t) * p.v_node + (int64_t)w.kvh * p.v_head;
-        take([&](int e) { return to_f32(k[e]); }, [&](int e) { return to_f32(v[e]); });
-    }
-    if (w.slot >= 0) {
-        const int64_t at = (int64_t)(w.slot + node - w.node0) * H + head;
-        if (lane == 0) p.part_ml[at] = make_float2(m, l);
-        for (int i = 0; i < 4; i++)
-            if (lane + 32 * i < dv) p.part_o[at * p.part_width + lane + 32 * i] = o[i];
-    } else {
-        const float M = p.sink ? fmaxf(m, 0.f) : m, x = exp2f(m - M), total = l * x + (p.sink ? exp2f(-M) : 0.f);
-        for (int i = 0; i < 4; i++)
-            if (lane + 32 * i < dv) static_cast<T*>(p.out)[((int64_t)node * H + head) * dv + lane + 32 * i] = from_f32<T>(total == 0.f ? 0.f : o[i] * x / total);
-    }
-}
 
 template <typename T, int DK, int DV>
 __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_constant__ DraftParams p, const __grid_constant__ CUtensorMap q_map,
@@ -539,7 +491,8 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
             const uint32_t again = __ballot_sync(0xffffffffu, active && !(fabsf(sum_a) + fabsf(sum_b) + l < INFINITY));
             if (again) {
                 __syncwarp();  // the rows above have been stored
-                for (uint32_t rest = again; rest; rest &= rest - 1) row_again<T>(p, w, warp * 32 + __ffs(rest) - 1, lane);
+                const DraftItem it = {w.node0, w.n_nodes, w.list, w.n_context, w.slot, w.tree, w.n_drafted, 0, {}};
+                for (uint32_t rest = again; rest; rest &= rest - 1) row_again<T>(p, it, w.kvh, warp * 32 + __ffs(rest) - 1, lane);
             }
             mbar_arrive(work_empty + 8 * (n & 1));
         }
