@@ -19,6 +19,7 @@ from torch import nn
 import chunk_attn
 from chunk_attn import ops
 
+from ..sequence import Sequence
 from .configuration_llama import LlamaConfig
 
 
@@ -91,6 +92,13 @@ class LlamaChunkAttention(nn.Module):
         out = kv_cache.forward(q=q)  # [n_seqs, H, d]
         return self.o_proj(out.view(-1, self.hidden_size))
 
+    def draft(self, hidden_states, batch, positions, cos_sin_cache, kv_cache):
+        """hidden_states [n_nodes, hidden] of drafted trees.  Returns (output, k, v): nothing is in the cache until
+        `Attention.extend_kv` brings the tokens that are accepted."""
+        q, k, v = self.qkv(hidden_states, positions, cos_sin_cache)
+        out = kv_cache.forward_draft(q, k, v, batch)
+        return self.o_proj(out.view(-1, self.hidden_size)), k, v
+
 
 class LlamaMLP(nn.Module):
     def __init__(self, config: LlamaConfig):
@@ -124,6 +132,12 @@ class LlamaDecoderLayer(nn.Module):
             kv_cache.refresh_kernel_context(force=False)
         return hidden_states, residual
 
+    def draft(self, hidden_states, residual, batch, positions, cos_sin_cache, kv_cache):
+        hidden_states, residual = self.input_layernorm(hidden_states, residual)
+        hidden_states, k, v = self.self_attn.draft(hidden_states, batch, positions, cos_sin_cache, kv_cache)
+        hidden_states, residual = self.post_attention_layernorm(hidden_states, residual)
+        return self.mlp(hidden_states), residual, k, v
+
 
 class LlamaModel(nn.Module):
     def __init__(self, config: LlamaConfig):
@@ -143,8 +157,9 @@ class LlamaModel(nn.Module):
                                                     self.config.rope_theta, w.dtype, w.device)
         return self.cos_sin_cache
 
-    def forward(self, seqs, kv_caches, prefill):
-        """Returns the final hidden state of each sequence's last real token, [n_seqs, hidden]."""
+    def forward(self, seqs, kv_caches, prefill, every_token=False):
+        """Returns the final hidden state of each sequence's last real token, [n_seqs, hidden]; of a prefill with every_token,
+        those of all tokens, padded ones included, [n_seqs, longest, hidden]."""
         device = self.norm.weight.device
         table = self._rope_table()
         if prefill:
@@ -167,10 +182,37 @@ class LlamaModel(nn.Module):
             hidden_states, residual = layer(hidden_states, residual, seqs, positions, table,
                                             kv_caches[i] if kv_caches else None, prefill)
         hidden_states, _ = self.norm(hidden_states, residual)
-        if prefill:
+        if prefill and not every_token:
             last = torch.tensor([n - 1 for n in lens], dtype=torch.long, device=device)
             hidden_states = hidden_states[torch.arange(len(seqs), device=device), last]
         return hidden_states
+
+    def checked(self, tokens):
+        if tokens and not 0 <= min(tokens) <= max(tokens) < self.config.vocab_size:
+            raise ValueError("a token id is outside the vocabulary of %d" % self.config.vocab_size)
+        return tokens
+
+    def draft(self, seqs, trees, kv_caches):
+        """One step over drafted trees: trees[i] = (tokens, parents) of sequence i, whose first node is its last token.  Returns
+        (final hidden states [n_nodes, hidden], the batch, the nodes' tokens int32, [(k, v)] of every layer)."""
+        device = self.norm.weight.device
+        table = self._rope_table()
+        batch = chunk_attn.DraftBatch([parents for _, parents in trees], device)
+        positions = []
+        for seq, (_, parents) in zip(seqs, trees):
+            at = len(positions)
+            for p in parents:
+                positions.append(len(seq) - 1 if p < 0 else positions[at + p] + 1)
+        if max(positions) >= table.shape[0]:
+            raise ValueError("sequence exceeds max_position_embeddings=%d" % table.shape[0])
+        tokens = self.checked([t for ts, _ in trees for t in ts])
+        input_ids, positions = torch.tensor([tokens, positions], dtype=torch.long, device=device)
+        hidden_states, residual, kvs = self.embed_tokens(input_ids), None, []
+        for layer, cache in zip(self.layers, kv_caches):
+            hidden_states, residual, k, v = layer.draft(hidden_states, residual, batch, positions, table, cache)
+            kvs.append((k, v))
+        hidden_states, _ = self.norm(hidden_states, residual)
+        return hidden_states, batch, input_ids.to(torch.int32), kvs
 
     def detect_free_memory(self):
         """MB available for all layers' pools (reference modeling_llama.py:234-247)."""
@@ -220,6 +262,64 @@ class LlamaForCausalLM(nn.Module):
     @torch.inference_mode()
     def forward(self, seqs, kv_caches, prefill):
         return torch.argmax(self.logits(seqs, kv_caches, prefill), dim=-1).tolist()
+
+    @torch.inference_mode()
+    def decode_drafts(self, seqs, kv_caches, drafts, thresholds=None, top=1):
+        """One decode step that takes as many tokens as the model agrees with: drafts[i] = (tokens, parents) drafted below
+        sequence i's last token (parents -1: that token), possibly none.  A drafted token is accepted where it is the model's choice,
+        with thresholds (epsilon, delta) also where its log probability is at least min(log epsilon, log delta - entropy).  The
+        accepted tokens' keys and values go to the caches.  Returns, per sequence, its new tokens (one at least) and for each of
+        them (log probability, log probabilities of the top best tokens, their ids)."""
+        if not seqs:
+            return [], []
+        if len(drafts) != len(seqs) or any(len(ts) != len(ps) for ts, ps in drafts):
+            raise ValueError("one draft per sequence and one parent per drafted token are required")
+        # node 0 of every tree is the sequence's last token
+        trees = [([seq[-1]] + list(ts), [-1] + [p + 1 for p in ps]) for seq, (ts, ps) in zip(seqs, drafts)]
+        hidden_states, batch, tokens, kvs = self.model.draft(seqs, trees, kv_caches)
+        # what a node's token is worth stands in its parent's row; the first nodes' are known
+        first = torch.tensor(batch.first[:-1], dtype=torch.int32, device=tokens.device)[batch.row_of.long()]
+        rooted = batch.parents < 0
+        lp, entropy, best_lp, best = chunk_attn.ops.token_log_probs(
+            self.lm_head(hidden_states), torch.where(rooted, -1, tokens), torch.where(rooted, 0, first + batch.parents),
+            max(1, min(top, self.config.vocab_size)))
+        choice = best[:, 0].contiguous()
+        if thresholds is None:
+            path, _, following = chunk_attn.ops.accept_draft(batch, tokens, choice)
+        else:
+            path, _, following = chunk_attn.ops.accept_draft(batch, tokens, choice, lp, entropy, *thresholds)
+        path, following = path.tolist(), following.tolist()
+        lines = [[batch.first[r] + n for n in line if n >= 0] for r, line in enumerate(path)]
+        # every accepted node's key and value, the first nodes' among them
+        kept = torch.tensor([n for line in lines for n in line], dtype=torch.long, device=tokens.device)
+        ids = [t for ts, _ in trees for t in ts]
+        taken = [[ids[n] for n in line] for line in lines]
+        rows = list(range(len(seqs)))
+        for cache, (k, v) in zip(kv_caches, kvs):
+            cache.extend_kv(rows, taken, k[kept], v[kept])
+        new = [t[1:] + [n] for t, n in zip(taken, following)]
+        own = torch.cat([lp, best_lp[:, 0]]).tolist()
+        best_lp, best = best_lp[:, :top].tolist(), best[:, :top].tolist()
+        # token j follows node j of the line: an accepted one's log probability is its node's, the last one is the last node's choice
+        told = [[(own[n], best_lp[up], best[up]) for n, up in zip(line[1:] + [len(tokens) + line[-1]], line)] for line in lines]
+        return new, told
+
+    @torch.inference_mode()
+    def score(self, prompts, top=0, portion=1024):
+        """Of every prompt (a list of token ids) and every token but its first: (log probabilities [n - 1], entropy of the
+        distributions that they were taken from [n - 1], top best tokens' log probabilities and ids [n - 1, top]).  portion: rows of
+        logits at a time."""
+        if not prompts or min(len(p) for p in prompts) < 1 or portion < 1:
+            raise ValueError("score needs prompts of at least one token and a positive portion")
+        seqs = [Sequence(self.model.checked(list(p))) for p in prompts]
+        hidden_states = self.model(seqs, None, prefill=True, every_token=True)
+        out = []
+        for row, prompt in zip(hidden_states, prompts):
+            targets = torch.tensor(prompt[1:], dtype=torch.int32, device=row.device)
+            parts = [chunk_attn.ops.token_log_probs(self.lm_head(row[i:min(i + portion, len(targets))]), targets[i:i + portion], None, top)
+                     for i in range(0, max(1, len(targets)), portion)]
+            out.append(tuple(torch.cat(x) for x in zip(*parts)))
+        return out
 
     def create_kv_caches(self):
         return self.model.create_kv_caches()

@@ -14,12 +14,18 @@ import threading
 
 import torch
 
+from chunk_attn import ops
+
 from ..logger import logger
 from .sequence import Sequence
 
 
 class ModelHost:
-    def __init__(self, model_obj, kv_caches, max_batch_size=32):
+    def __init__(self, model_obj, kv_caches, max_batch_size=32, draft=None, thresholds=None):
+        """draft(tokens, depth) -> (drafted tokens, parents): decode steps check drafted tokens, for models with
+        `decode_drafts`; thresholds as there."""
+        if draft is not None and not hasattr(model_obj, "decode_drafts"):
+            raise ValueError("%s does not decode drafted tokens" % type(model_obj).__name__)
         self.model_obj = model_obj
         self.kv_caches = kv_caches
         self.running_seqs = []
@@ -29,18 +35,23 @@ class ModelHost:
         self.cycle_time = 1.0
         self.failure = None
         self.n_decode_steps = 0
+        self.draft, self.thresholds = draft, thresholds
+        self.n_drafted = self.n_accepted = 0
         self.batch_queue = queue.Queue(maxsize=2 * max_batch_size)
         self.thread = None
 
     # ---- client side ---------------------------------------------------------------------------
-    def predict_async(self, prompt_tokens, max_tokens):
+    def predict_async(self, prompt_tokens, max_tokens, log_probs=None):
+        """log_probs: k >= 0, also keep every generated token's log probability and the k best tokens (`Sequence`)."""
         if self.failure is not None:
             raise RuntimeError("model host failed: %r" % (self.failure,))
         if self.stopped:
             raise RuntimeError("model host is stopped, can't predict anymore")
         if len(prompt_tokens) == 0:
             raise ValueError("empty prompt")
-        seq = Sequence(prompt_tokens=prompt_tokens, max_tokens=max_tokens)
+        if log_probs is not None and not 0 <= log_probs <= 32:
+            raise ValueError("log_probs must be 0 to 32")
+        seq = Sequence(prompt_tokens=prompt_tokens, max_tokens=max_tokens, log_probs=log_probs)
         self.batch_queue.put(seq)
         return seq
 
@@ -99,13 +110,43 @@ class ModelHost:
         self.running_seqs = kept
         return n_removed
 
+    def next_tokens(self, seqs, prefill):
+        """The model's next token of each sequence; where log probabilities are asked for, those too."""
+        top = max((s.log_probs for s in seqs if s.log_probs is not None), default=None)
+        if top is None:
+            return self.model_obj(seqs, self.kv_caches, prefill=prefill)
+        logits = self.model_obj.logits(seqs, self.kv_caches, prefill)
+        _, _, best_lp, best = ops.token_log_probs(logits, top=max(1, min(top, logits.shape[1])))
+        best_lp, best = best_lp.tolist(), best.tolist()
+        for seq, lps, ids in zip(seqs, best_lp, best):
+            if seq.log_probs is not None:
+                seq.token_log_probs.append((lps[0], lps[:seq.log_probs], ids[:seq.log_probs]))
+        return [ids[0] for ids in best]
+
+    def decode_drafts(self):
+        """One decode step over drafted tokens.  The draft is asked for lines that end with the sequence; what a longer one brings
+        beyond its end is dropped."""
+        seqs = self.running_seqs
+        drafts = [self.draft(s.tokens, s.max_tokens + len(s.prompt_tokens) - len(s) - 1) for s in seqs]
+        top = max((s.log_probs for s in seqs if s.log_probs is not None), default=0)
+        new, told = self.model_obj.decode_drafts(seqs, self.kv_caches, drafts, self.thresholds, top)
+        for seq, (drafted, _), tokens, about in zip(seqs, drafts, new, told):
+            self.n_drafted += len(drafted)
+            self.n_accepted += len(tokens) - 1
+            for token, (lp, lps, ids) in zip(tokens, about):
+                if seq.finished():
+                    break
+                seq.append(token)
+                if seq.log_probs is not None:
+                    seq.token_log_probs.append((lp, lps[:seq.log_probs], ids[:seq.log_probs]))
+
     def step(self):
         """One iteration of the serving loop; returns the number of sequences that were decoded."""
         self.retire_finished()
         arrived = self.get_new_requests()
         if arrived:
             logger.debug("prefill of %d new seqs, %d running", len(arrived), len(self.running_seqs))
-            new_tokens = self.model_obj(arrived, self.kv_caches, prefill=True)
+            new_tokens = self.next_tokens(arrived, prefill=True)
             for seq, tok in zip(arrived, new_tokens):
                 seq.append(tok)
             for seq in arrived:  # same order as the caches inserted them: rows stay aligned
@@ -116,9 +157,11 @@ class ModelHost:
         if len(live) != len(self.running_seqs):
             self.retire_finished()
         if self.running_seqs:
-            new_tokens = self.model_obj(self.running_seqs, self.kv_caches, prefill=False)
-            for seq, tok in zip(self.running_seqs, new_tokens):
-                seq.append(tok)
+            if self.draft is not None:
+                self.decode_drafts()
+            else:
+                for seq, tok in zip(self.running_seqs, self.next_tokens(self.running_seqs, prefill=False)):
+                    seq.append(tok)
             self.n_decode_steps += 1
         return len(self.running_seqs)
 

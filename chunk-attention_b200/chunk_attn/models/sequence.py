@@ -8,13 +8,16 @@ _ids = itertools.count()
 class Sequence:
     """Prompt + generated tokens.  `index` is the row the sequence occupies in the KV caches' DFS
     order (set by the model's prefill); `get_result()` blocks until the host marks it finished or
-    failed."""
+    failed.  With `log_probs` = k, `token_log_probs` has (log probability, the k best tokens' log probabilities, their ids) of every
+    generated token."""
 
-    def __init__(self, prompt_tokens, max_tokens=2048):
+    def __init__(self, prompt_tokens, max_tokens=2048, log_probs=None):
         self.id = "seq-%d" % next(_ids)
         self.prompt_tokens = list(prompt_tokens)
         self.max_tokens = max_tokens
         self.tokens = list(self.prompt_tokens)
+        self.log_probs = log_probs
+        self.token_log_probs = []
         self.index = None
         self.error = None
         self.result_ready = threading.Event()

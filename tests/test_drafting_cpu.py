@@ -1,0 +1,105 @@
+"""Drafts from a sequence's own text, and the host's decode steps over drafts, without a GPU."""
+import random
+
+import pytest
+
+import test_model_host_cpu as H
+from chunk_attn.models.drafting import PromptLookup
+from chunk_attn.models.model_host import ModelHost
+
+
+def test_prompt_lookup():
+    look = PromptLookup(n_tokens=4, ngram=2, lines=1)
+    assert look([1, 2, 3, 4, 9, 1, 2], 8) == ([3, 4, 9, 1], [-1, 0, 1, 2])
+    assert look([1, 2, 3, 4, 9, 1, 2], 2) == ([3, 4], [-1, 0])
+    assert look([1, 2, 3], 8) == ([], []) and look([5], 8) == ([], []) and look([1, 1], 0) == ([], [])
+    assert look([7, 7], 8) == ([7], [-1])
+    two = PromptLookup(n_tokens=6, ngram=2, lines=2)
+    # "1 2" stood twice before: 3 4 .. last, 3 5 .. first; they share 3
+    tokens, parents = two([1, 2, 3, 5, 6, 1, 2, 3, 4, 8, 1, 2], 3)
+    assert tokens == [3, 4, 8, 5, 6] and parents == [-1, 0, 1, 0, 3]
+    for bad in ((0, 1, 1), (256, 1, 1), (1, 0, 1), (1, 1, 0)):
+        with pytest.raises(ValueError):
+            PromptLookup(*bad)
+
+
+def test_drafts_are_trees_of_the_text():
+    rng = random.Random(0)
+    for _ in range(200):
+        tokens = [rng.randrange(4) for _ in range(rng.randint(1, 40))]
+        look = PromptLookup(rng.randint(1, 9), rng.randint(1, 4), rng.randint(1, 3))
+        depth = rng.randint(0, 9)
+        drafted, parents = look(tokens, depth)
+        assert len(drafted) == len(parents) <= look.n_tokens
+        assert len(set(zip(parents, drafted))) == len(drafted)
+        deep = []
+        for i, p in enumerate(parents):
+            assert -1 <= p < i
+            deep.append(1 if p < 0 else deep[p] + 1)
+        assert max(deep, default=0) <= depth
+
+
+class DraftingModel(H.TreeModel):
+    """Takes drafted tokens as the decoder does: the longest line that its own next tokens agree with."""
+
+    def decode_drafts(self, seqs, kv_caches, drafts, thresholds, top):
+        for cache in kv_caches:
+            assert H.tree_rows(cache.tree) == [s.tokens[:-1] for s in seqs]
+        new = []
+        for r, (seq, (tokens, parents)) in enumerate(zip(seqs, drafts)):
+            line, kept = -1, []
+            while True:
+                want = H.next_token(seq.tokens + kept)
+                step = [i for i in range(len(tokens)) if parents[i] == line and tokens[i] == want]
+                if not step:
+                    break
+                line = step[0]
+                kept.append(want)
+            new.append(kept + [want])
+            for cache in kv_caches:
+                cache.tree.extend_seq(r, [seq[-1]] + kept)
+        return new, [[(0.0, [], [])] * len(t) for t in new]
+
+
+@pytest.mark.parametrize("batch", [1, 3])
+def test_host_over_drafts(batch):
+    """Every request's tokens are those of plain decoding, in fewer steps when the drafts are right, whatever the drafts are."""
+    rng = random.Random(1)
+    prompts = [[rng.randrange(1000) for _ in range(n)] for n in (3, 9, 4, 17, 8)]
+    lens = [12, 1, 30, 7, 19]
+    truth = {tuple(p): H.rollout(p, 40) for p in prompts}
+
+    def oracle(tokens, depth):  # a right line of three, and a wrong one beside it
+        rest = next(t for p, t in truth.items() if tuple(t[:len(tokens)]) == tuple(tokens))[len(tokens):][:min(3, depth)]
+        return rest + [5], list(range(-1, len(rest) - 1)) + [-1]
+
+    steps = []
+    for draft in (lambda t, d: ([], []), lambda t, d: ([1, 2], [-1, 0]) if d > 1 else ([], []), oracle):
+        caches = [H.TreeCache(), H.TreeCache()]
+        host = ModelHost(DraftingModel(), caches, max_batch_size=batch, draft=draft)
+        host.cycle_time = 0.02
+        with host:
+            seqs = [host.predict_async(p, n) for p, n in zip(prompts, lens)]
+            for seq, p, n in zip(seqs, prompts, lens):
+                assert seq.get_result(timeout=60) == H.rollout(p, n)
+        steps.append(host.n_decode_steps)
+    assert steps[0] == steps[1] and steps[2] < steps[0] / 2
+    assert host.n_accepted > 0 and host.n_drafted > host.n_accepted
+
+
+def test_a_draft_beyond_the_end_is_cut():
+    caches = [H.TreeCache()]
+    host = ModelHost(DraftingModel(), caches, max_batch_size=2, draft=lambda t, depth: (H.rollout(t, 9)[len(t):], list(range(-1, 8))))
+    host.cycle_time = 0.02
+    with host:
+        for n in (1, 2, 4, 13):
+            assert host.predict([4, 5, 6], n) == H.rollout([4, 5, 6], n)
+
+
+def test_host_refuses():
+    with pytest.raises(ValueError, match="does not decode drafted"):
+        ModelHost(H.TreeModel(), [], draft=PromptLookup())
+    host = ModelHost(H.TreeModel(), [H.TreeCache()])
+    host.stopped = False
+    with pytest.raises(ValueError, match="log_probs"):
+        host.predict_async([1], 1, log_probs=33)
