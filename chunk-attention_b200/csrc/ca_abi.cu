@@ -1809,6 +1809,8 @@ int ca_draft_attention(ca_context* c, const ca_draft_args* a, ca_stream stream_)
     if (reinterpret_cast<uintptr_t>(a->out) % 16 || reinterpret_cast<uintptr_t>(a->work) % 16 || reinterpret_cast<uintptr_t>(a->seen) % 8 ||
         reinterpret_cast<uintptr_t>(a->partials) % 16)
         return fail(CA_ERR_INVALID, "drafted tokens: out, work list and scratch must be 16-byte aligned");
+    for (const void* t : {a->q, a->k, a->v})
+        if (reinterpret_cast<uintptr_t>(t) % c->geo.esize) return fail(CA_ERR_INVALID, "drafted tokens: q, k and v must be aligned to their type");
     if ((int64_t)a->info->n_items * c->geo.n_heads > INT32_MAX || (int64_t)a->info->n_nodes * c->geo.n_heads * c->group > INT32_MAX - 4) return fail(CA_ERR_INVALID, "drafted tokens: too many pieces of work");
     DeviceGuard guard(c->device);
     if (guard.err != cudaSuccess) return fail_cuda(guard.err, "cudaSetDevice");
@@ -1880,6 +1882,9 @@ int ca_accept_draft(const ca_accept_args* a, ca_stream stream) {
     if (a->words < 1 || a->words > CA_DRAFT_MAX_NODES / 32) return fail(CA_ERR_INVALID, "accept_draft: words must be 1 to 8");
     if ((a->log_probs == nullptr) != (a->entropy == nullptr)) return fail(CA_ERR_INVALID, "accept_draft: log_probs and entropy come together");
     if (a->log_probs && !(a->epsilon > 0 && a->delta > 0)) return fail(CA_ERR_INVALID, "accept_draft: epsilon and delta must be positive");
+    for (const void* t : {(const void*)a->first, (const void*)a->parent, (const void*)a->depth, (const void*)a->seen, (const void*)a->tokens, (const void*)a->choice,
+                          (const void*)a->log_probs, (const void*)a->entropy, (const void*)a->path, (const void*)a->count, (const void*)a->next})
+        if (reinterpret_cast<uintptr_t>(t) % 4) return fail(CA_ERR_INVALID, "accept_draft: an operand is not 4-byte aligned");
     ca::AcceptParams p{};
     p.first = a->first;
     p.parent = a->parent;
@@ -1920,6 +1925,10 @@ int ca_token_log_probs(const ca_log_probs_args* a, ca_stream stream) {
     if (a->n_rows > 0 && (!a->logits || !a->entropy || !a->scratch)) return fail(CA_ERR_INVALID, "token_log_probs: null operand");
     if (a->n_tokens > 0 && (!a->tokens || !a->log_probs)) return fail(CA_ERR_INVALID, "token_log_probs: null operand");
     if (a->n_rows > 0 && a->top > 0 && (!a->top_ids || !a->top_log_probs)) return fail(CA_ERR_INVALID, "token_log_probs: null operand");
+    if (reinterpret_cast<uintptr_t>(a->logits) % shaped_esize_of(a->dtype) || reinterpret_cast<uintptr_t>(a->scratch) % 16)
+        return fail(CA_ERR_INVALID, "token_log_probs: logits must be aligned to their type, scratch to 16 bytes");
+    for (const void* t : {(const void*)a->tokens, (const void*)a->rows, (const void*)a->log_probs, (const void*)a->entropy, (const void*)a->top_log_probs, (const void*)a->top_ids})
+        if (reinterpret_cast<uintptr_t>(t) % 4) return fail(CA_ERR_INVALID, "token_log_probs: an operand is not 4-byte aligned");
     ca::LogProbsParams p{};
     p.logits = a->logits;
     p.row_stride = a->row_stride;

@@ -528,7 +528,8 @@ CA_API int64_t ca_scan_scratch_floats(const ca_spans* spans, int channels, int n
 CA_API int ca_selective_scan(void* y, const void* x, const void* z, int64_t z_stride, const float* dt, const float* dt_bias,
                              const float* A, const float* bc, int64_t bc_stride, const float* D, float* state, float* scratch,
                              const ca_spans* spans, int channels, int n_states, int dtype, ca_stream stream);
-/* 0, or 1 when a bounded wait inside a block kernel of the current device has run out (synchronises the stream) */
+/* 0, or 1 when a bounded wait inside a block kernel or that of ca_token_log_probs on the current device has run out (synchronises
+ * the stream) */
 CA_API int ca_block_status(int32_t* status, ca_stream stream);
 CA_API int64_t ca_decay_scratch_floats(const ca_spans* spans, int n_heads, int d_key, int d_value, int dtype);
 CA_API int ca_decay_attention(void* out, const void* qkv, int64_t row_stride, const float* decay, float* state, float* scratch,
@@ -707,7 +708,8 @@ CA_API int ca_accept_draft(const ca_accept_args* args, ca_stream stream);
  * log_probs[i] = logits[rows[i]][tokens[i]] - lse (rows NULL: i; token -1: 0; other ids or rows out of range: NaN),
  * entropy[r] = lse - sum p x, and the top best tokens of a row by value, of equal ones those with the lowest ids:
  * top_ids, top_log_probs [n_rows, top].  Excluded tokens (-infinity) have probability 0.  A row that holds a NaN, +infinity or nothing
- * but -infinity has no distribution: its numbers are NaN (top_ids counts NaN as -infinity).  scratch: ca_log_probs_scratch bytes. */
+ * but -infinity has no distribution: its numbers are NaN (top_ids counts NaN as -infinity).  scratch: ca_log_probs_scratch bytes,
+ * 16-byte aligned. */
 #define CA_MAX_TOP 32
 typedef struct ca_log_probs_args {
     const void* logits;

@@ -1,4 +1,5 @@
 """Drafted tokens without a GPU: the batch's tables, its refusals, and the work list, walked in numpy as the kernels walk it."""
+import ctypes as C
 import math
 import random
 
@@ -129,3 +130,48 @@ def test_work_lists_refuse():
         cabi.DraftPlan(ok, [0, 2], kv_heads=0)
     assert cabi.DraftPlan([], [0]).info.n_items == 0
     assert cabi.DraftPlan([], [0, 0]).info.n_items == 0
+
+
+class AcceptArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("first", "parent", "depth", "seen")] + [(n, C.c_int32) for n in ("words", "n_rows", "width")] + \
+        [(n, C.c_void_p) for n in ("tokens", "choice", "log_probs", "entropy")] + [("epsilon", C.c_double), ("delta", C.c_double)] + \
+        [(n, C.c_void_p) for n in ("path", "count", "next")]
+
+
+class LogProbsArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_int64)] + [(n, C.c_int32) for n in ("n_rows", "vocab", "dtype")] + \
+        [("tokens", C.c_void_p), ("rows", C.c_void_p), ("n_tokens", C.c_int32), ("top", C.c_int32)] + \
+        [(n, C.c_void_p) for n in ("log_probs", "entropy", "top_log_probs", "top_ids", "scratch")]
+
+
+def refused(fn, args, what):
+    assert fn(C.byref(args), None) != cabi.CA_OK and what in cabi.lib.ca_last_error().decode()
+
+
+def test_acceptance_refuses_at_the_c_entry():
+    """Every call is refused before anything is launched: the addresses are never followed."""
+    ok = {n: 4096 for n, t in AcceptArgs._fields_ if t is C.c_void_p}
+    ok.update(words=2, n_rows=1, width=1, epsilon=0.1, delta=0.3)
+    for name in ("first", "parent", "depth", "seen", "tokens", "choice", "path", "count", "next"):
+        refused(cabi.lib.ca_accept_draft, AcceptArgs(**dict(ok, **{name: 0})), "null")
+        refused(cabi.lib.ca_accept_draft, AcceptArgs(**dict(ok, **{name: 4098})), "aligned")
+    for change, what in (({"n_rows": -1}, "negative"), ({"width": -1}, "negative"), ({"words": 0}, "words"), ({"words": 9}, "words"), ({"entropy": 0}, "together"),
+                         ({"log_probs": 0}, "together"), ({"epsilon": 0.0}, "positive"), ({"delta": float("nan")}, "positive"), ({"entropy": 4097}, "aligned")):
+        refused(cabi.lib.ca_accept_draft, AcceptArgs(**dict(ok, **change)), what)
+    assert cabi.lib.ca_accept_draft(C.byref(AcceptArgs(**dict(ok, n_rows=0))), None) == cabi.CA_OK
+    assert cabi.lib.ca_accept_draft(None, None) != cabi.CA_OK
+
+
+def test_log_probs_refuse_at_the_c_entry():
+    ok = {n: 4096 for n, t in LogProbsArgs._fields_ if t is C.c_void_p}
+    ok.update(row_stride=100, n_rows=2, vocab=100, dtype=cabi.CA_DTYPE_F32, n_tokens=2, top=3)
+    for name in ("logits", "entropy", "scratch", "tokens", "log_probs", "top_ids", "top_log_probs"):
+        refused(cabi.lib.ca_token_log_probs, LogProbsArgs(**dict(ok, **{name: 0})), "null")
+        refused(cabi.lib.ca_token_log_probs, LogProbsArgs(**dict(ok, **{name: 4098})), "aligned")
+    for change, what in (({"n_rows": -1}, "sizes"), ({"n_tokens": -1}, "sizes"), ({"vocab": 0}, "sizes"), ({"vocab": (1 << 28) + 1}, "2^28"), ({"dtype": 9}, "fp16"),
+                         ({"top": -1}, "top"), ({"top": 33}, "top"), ({"top": 101}, "top"), ({"vocab": 2}, "top"), ({"row_stride": -1}, "stride"), ({"rows": 4097}, "aligned"),
+                         ({"scratch": 4104}, "scratch")):
+        refused(cabi.lib.ca_token_log_probs, LogProbsArgs(**dict(ok, **change)), what)
+    assert cabi.lib.ca_token_log_probs(None, None) != cabi.CA_OK
+    for bad in ((-1, 10, cabi.CA_DTYPE_F32, 1), (1, 0, cabi.CA_DTYPE_F32, 1), (1, 10, 9, 1), (1, 10, cabi.CA_DTYPE_F32, 33)):
+        assert cabi.lib.ca_log_probs_scratch(*bad) < 0

@@ -16,7 +16,7 @@ from chunk_attn.models.model_host import ModelHost
 from chunk_attn.models.registry import load_model
 from chunk_attn.models.sequence import Sequence
 from llama_dense import dense_logits
-from test_gpu_model_folders import write_folder
+from test_gpu_model_folders import gagorax_folder, reference, tokens_for, write_folder  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -236,3 +236,24 @@ def test_command(tmp_path, monkeypatch, capsys):
     for bad in (["--draft-tokens", "-1"], ["--draft-tokens", "256"], ["--log-probs", "33"]):
         with pytest.raises(SystemExit):
             generate.main(["--model", str(tmp_path)] + bad)
+
+
+def test_log_probs_of_a_model_without_drafts(gagorax_folder, monkeypatch, capsys):  # noqa: F811
+    """The host takes log probabilities from any model's scores; drafts are refused where the model has no step for them."""
+    cfg, w, path = gagorax_folder
+    prompts = [tokens_for(cfg, n, n) for n in (3, 70)]
+    text = "\n".join(" ".join(map(str, p)) for p in prompts) + "\n"
+    args = ["--model", str(path / "m"), "--dtype", "float32", "--max-new-tokens", "5"]
+    monkeypatch.setattr(sys, "stdin", io.StringIO(text))
+    assert generate.main(args + ["--log-probs", "2"]) == 0
+    lines = capsys.readouterr().out.splitlines()
+    for p, line, about in zip(prompts, lines[::2], lines[1::2]):
+        toks = [int(t) for t in line.split()]
+        ref = torch.log_softmax(torch.tensor(reference(cfg, w, toks)).double(), -1)
+        for t, (lp, lps, ids) in enumerate(json.loads(about)):
+            row = ref[len(p) - 1 + t]
+            # the scores themselves are compared to 1e-3 where this model is tested
+            assert ids[0] == toks[len(p) + t] and abs(lp - row[ids[0]].item()) < 1e-3 and max(abs(l - row[i].item()) for l, i in zip(lps, ids)) < 1e-3
+    monkeypatch.setattr(sys, "stdin", io.StringIO(text))
+    with pytest.raises(ValueError, match="does not decode drafted"):
+        generate.main(args + ["--draft-tokens", "2"])
