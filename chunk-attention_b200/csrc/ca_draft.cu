@@ -779,13 +779,14 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_tf32_kernel(const __grid_c
     }
 }
 
+constexpr int MOST_SHARED = 232448;  // of a CTA
+
 template <typename T>
 cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t stream) {
     const GenericSizes z = generic_sizes(p.d_key, p.d_value, sizeof(T));
     auto go = [&](auto* k, int threads, size_t floats) {
         const size_t smem = whole((int)(sizeof(float) * floats), 128) + (size_t)G_STAGES * z.stage();
-        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        const cudaError_t e = allow_shared(reinterpret_cast<const void*>(k), MOST_SHARED - 128);  // less the barriers; other head sizes take other amounts
         if (e != cudaSuccess) return e;
         return launch_kernel(k, dim3((unsigned)p.n_items * p.geo.n_heads), threads, smem, 1, p.dependent & DEPENDENT_ATTENTION, stream, p, z);
     };
@@ -946,7 +947,7 @@ __global__ void __launch_bounds__(32) accept_draft_kernel(const AcceptParams p) 
 int draft_generic_ctas(int block_rows, int dk, int dv, int esize) {
     const GenericSizes z = generic_sizes(dk, dv, esize);
     const int rows = sizeof(float) * block_rows * (z.q_floats + (block_rows <= 16 ? (G_WARPS + 1) * G_TOK + 3 : G_TOK));
-    return B200_SMS * std::max(1, std::min(2, 232448 / (rows + G_STAGES * z.stage() + 1024 + 128)));
+    return B200_SMS * std::max(1, std::min(2, MOST_SHARED / (rows + G_STAGES * z.stage() + 1024 + 128)));
 }
 
 cudaError_t launch_draft_generic(const DraftParams& p, int block_rows, int dtype, cudaStream_t stream) {

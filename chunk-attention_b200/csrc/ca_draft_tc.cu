@@ -536,8 +536,7 @@ cudaError_t launch(const DraftParams& p, cudaStream_t stream) {
         if (e != cudaSuccess) return e;
         ready = true;
     }
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    const cudaError_t e = allow_shared(reinterpret_cast<const void*>(k), smem);
     if (e != cudaSuccess) return e;
     return launch_kernel(k, dim3((unsigned)p.n_items * G), A_THREADS, smem, 1, p.dependent & DEPENDENT_ATTENTION, stream, p, qm, km, vm);
 }

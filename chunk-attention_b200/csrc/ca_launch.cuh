@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <cstdint>
 #include <cstdlib>
 
 namespace ca {
@@ -34,6 +36,28 @@ cudaError_t launch_kernel(void (*kernel)(P...), dim3 grid, int threads, size_t s
         cfg.numAttrs = n;
         e = cudaLaunchKernelEx(&cfg, kernel, args...);
     }
+    return e;
+}
+
+// Once per kernel and device: room for smem bytes of dynamic shared memory, and all of an SM's for it (set at every launch otherwise, for nothing;
+// a full table only costs that).
+inline cudaError_t allow_shared(const void* kernel, int smem) {
+    struct Slot { std::atomic<const void*> kernel{nullptr}; std::atomic<uint64_t> devices{0}; };
+    static Slot slots[256];
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    Slot* at = nullptr;
+    size_t i = reinterpret_cast<uintptr_t>(kernel) / 16 % 256;
+    for (int n = 0; n < 256 && !at; n++, i = (i + 1) % 256) {
+        const void* have = slots[i].kernel.load(std::memory_order_relaxed);
+        if (have == kernel || (!have && (slots[i].kernel.compare_exchange_strong(have, kernel) || have == kernel))) at = &slots[i];
+    }
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (at && (at->devices.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess && at) at->devices.fetch_or(bit, std::memory_order_release);
     return e;
 }
 

@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(L_THREADS, 4) log_probs_kernel(const LogProbsP
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    // Every wait is bounded: on expiry the status is recorded, and no later one waits
+    // Every wait is bounded: on expiry the status is recorded, no later one waits, and thread 0 sees its copies in flight land
     long long patience = L_WAIT_LIMIT;
     auto wait = [&](uint32_t bar, int parity) {
         if (ptx::mbar_wait_bounded(bar, parity, patience)) return;
@@ -432,6 +432,10 @@ __global__ void __launch_bounds__(L_THREADS, 4) log_probs_kernel(const LogProbsP
         ptx::bulk_copy_g2s(stages + stage * L_STEP * 16, ahead.at(ahead_b), bytes, full + 8 * stage);
         ahead_b += L_STEP;
         asked++;
+    };
+    auto drain = [&] {
+        if (tid == 0 && patience == 0)
+            for (int i = max(0, asked - L_STAGES); i < asked; i++) ptx::mbar_wait_bounded(full + 8 * (i % L_STAGES), (i / L_STAGES) & 1, L_WAIT_LIMIT);
     };
     if (tid == 0) {
         ask();
@@ -562,12 +566,16 @@ __global__ void __launch_bounds__(L_THREADS, 4) log_probs_kernel(const LogProbsP
                 for (int i = tid; i < min(hits, L_HITS); i += L_THREADS) to.hits[i] = sh.hits[place][i];
             }
             turn_at = ((int64_t)s.row + 1) * p.turns;
-            if (turn_at >= turn_end) return;
+            if (turn_at >= turn_end) {
+                drain();
+                return;
+            }
             s = stretch(turn_at);
             continue;
         }
 
         // ---- a cluster finishes its row
+        drain();
         Best best = {-INFINITY, NO_ID};
         if (TOP) {
             const int lo = s.first ? 0 : s.head + s.v0 * N, hi = s.last ? p.vocab : s.head + s.v1 * N, hits = sh.n_hits[0];
@@ -727,10 +735,7 @@ __global__ void __launch_bounds__(128) given_tokens_kernel(const LogProbsParams 
 
 template <typename T>
 cudaError_t launch(const LogProbsParams& p, cudaStream_t stream) {
-    auto with_ring = [](auto* k) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, L_RING);
-        return e == cudaSuccess ? cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) : e;
-    };
+    auto with_ring = [](auto* k) { return allow_shared(reinterpret_cast<const void*>(k), L_RING); };
     if (p.n_rows > 0) {
         cudaError_t e;
         if (p.splits > 0) {

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <chrono>
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -593,7 +594,7 @@ torch::Tensor Attention::forward_draft(torch::Tensor q, torch::Tensor k, torch::
     if (!fits(q, n_heads_, d_head_) || !fits(k, kv_heads(), d_head_) || !fits(v, kv_heads(), dv))
         throw std::runtime_error("forward_draft: q must be [n_nodes, n_heads, d_key], k and v [n_nodes, n_kv_heads, .] with the dtype and device of the cache and contiguous heads");
     c10::cuda::CUDAGuard guard(options_.device());
-    torch::Tensor out = torch::empty({n, n_heads_, dv}, options_);
+    torch::Tensor out = at::detail::empty_cuda({n, n_heads_, dv}, st, options_.device(), c10::nullopt);
     if (n == 0) return out;
     if (!draft_ || draft_->serial != draft.serial() || draft_version_ != tree_->version() || draft_appended_ != tree_->appended()) {
         std::vector<ca_chunk_info> infos = tree_->get_chunks();
@@ -645,7 +646,7 @@ torch::Tensor Attention::forward_draft(torch::Tensor q, torch::Tensor k, torch::
     torch::Tensor scratch;
     const int64_t floats = ca_draft_partial_floats(ctx_, a.info);
     if (floats > 0) {
-        scratch = torch::empty({floats}, options_.dtype(torch::kFloat32));
+        scratch = scratch_on(options_.device(), torch::kFloat32, floats);
         a.partials = scratch.data_ptr<float>();
     }
     check_rc(ca_draft_attention(ctx_, &a, stream()), "forward_draft");

@@ -2,6 +2,7 @@
 // call the C ABI on torch's current stream.
 #include "draft.h"
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -28,6 +29,15 @@ void check_rc(int rc, const char* what) {
     if (rc != CA_OK) throw std::runtime_error(std::string(what) + ": " + ca_last_error());
 }
 }  // namespace
+
+torch::Tensor scratch_on(torch::Device device, c10::ScalarType type, int64_t n) { return at::detail::empty_cuda({n}, type, device, c10::nullopt); }
+
+torch::Tensor part_of(const torch::Tensor& whole, c10::ScalarType type, int64_t at, c10::IntArrayRef sizes) {
+    torch::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+}
 
 bool capturing(torch::Device device) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
@@ -121,7 +131,7 @@ DraftBatch::DraftBatch(const std::vector<std::vector<int>>& trees, torch::Device
 
 DraftBatch::View DraftBatch::view(std::vector<torch::Tensor>* keep) {
     const int32_t* p = buffer_.use();
-    if (device_.is_cuda() && capturing(device_)) (keep ? *keep : captured_).push_back(buffer_.tensor());
+    if (keep && device_.is_cuda() && capturing(device_)) keep->push_back(buffer_.tensor());
     return {p + at_first_, p + at_parent_, p + at_depth_, reinterpret_cast<const uint32_t*>(p)};
 }
 
@@ -150,8 +160,9 @@ py::tuple accept_draft(DraftBatch& draft, Tensor tokens, Tensor choice, c10::opt
     }
     c10::cuda::CUDAGuard guard(dev);
     const int64_t width = draft.max_depth() + 1;
-    Tensor out = torch::empty({rows * (width + 2)}, torch::TensorOptions().dtype(torch::kInt32).device(dev));
-    Tensor path = out.narrow(0, 0, rows * width).view({rows, width}), count = out.narrow(0, rows * width, rows), next = out.narrow(0, rows * (width + 1), rows);
+    const Tensor out = scratch_on(dev, torch::kInt32, rows * (width + 2));
+    Tensor path = part_of(out, torch::kInt32, 0, {rows, width}), count = part_of(out, torch::kInt32, rows * width, {rows}),
+           next = part_of(out, torch::kInt32, rows * (width + 1), {rows});
     const auto view = draft.view();
     ca_accept_args a{};
     a.first = view.first;
@@ -193,12 +204,12 @@ py::tuple token_log_probs(Tensor logits, c10::optional<Tensor> tokens, c10::opti
         else need(asked == n, "token_log_probs: one token per row is required (or rows)");
     }
     c10::cuda::CUDAGuard guard(dev);
-    const auto f32 = torch::TensorOptions().dtype(torch::kFloat32).device(dev);
-    Tensor log_probs = torch::empty({asked}, f32), entropy = torch::empty({n}, f32), top_lp = torch::empty({n, top}, f32),
-           top_ids = torch::empty({n, top}, f32.dtype(torch::kInt32));
+    const Tensor out = scratch_on(dev, torch::kFloat32, asked + n + 2 * n * top);
+    Tensor log_probs = part_of(out, torch::kFloat32, 0, {asked}), entropy = part_of(out, torch::kFloat32, asked, {n}),
+           top_lp = part_of(out, torch::kFloat32, asked + n, {n, top}), top_ids = part_of(out, torch::kInt32, asked + n + n * top, {n, top});
     ca_log_probs_args a{};
     a.dtype = st == torch::kFloat16 ? CA_DTYPE_F16 : (st == torch::kFloat32 ? CA_DTYPE_F32 : CA_DTYPE_BF16);
-    Tensor scratch = torch::empty({std::max<int64_t>(1, ca_log_probs_scratch((int)n, (int)vocab, a.dtype, (int)top))}, f32.dtype(torch::kUInt8));
+    const Tensor scratch = scratch_on(dev, torch::kUInt8, std::max<int64_t>(1, ca_log_probs_scratch((int)n, (int)vocab, a.dtype, (int)top)));
     a.logits = logits.data_ptr();
     a.row_stride = n > 1 ? logits.stride(0) : vocab;
     a.n_rows = (int32_t)n;

@@ -24,6 +24,10 @@ class Uploaded {
     std::shared_ptr<at::cuda::CUDAEvent> ready_;
     c10::StreamId stream_ = 0;
 };
+// Outputs and scratch without the way through torch's dispatcher (accept_draft 8.2 -> 5.1 us a call, token_log_probs 9.0 -> 5.5 us of the host): a
+// tensor of n elements, and one over a part of another's memory, from element `at` of its own type on
+torch::Tensor scratch_on(torch::Device device, c10::ScalarType type, int64_t n);
+torch::Tensor part_of(const torch::Tensor& whole, c10::ScalarType type, int64_t at, c10::IntArrayRef sizes);
 bool capturing(torch::Device device);  // whether the current stream is being captured into a graph
 
 class DraftBatch {
@@ -52,7 +56,6 @@ class DraftBatch {
     std::vector<int32_t> first_, depths_;
     torch::Device device_;
     Uploaded buffer_;
-    std::vector<torch::Tensor> captured_;
     int64_t serial_;
     int64_t at_first_ = 0, at_parent_ = 0, at_depth_ = 0;
     int words_ = 2, max_depth_ = -1;
