@@ -135,30 +135,31 @@ struct Stages {
         const bool bulk = walk.fetch(t, stage, bars + 8 * stage);
         used = (used & ~(1u << stage)) | (bulk ? 1u << stage : 0u);
     }
-    // The tile of the stage is there, for the whole block.  False: a copy did not come in time; status is recorded
-    __device__ __forceinline__ bool wait(int stage) {
+    // The tiles of the stage and of n - 1 behind it are there, for the whole block.  False: a copy did not come in time; status is recorded
+    template <int N = 1> __device__ __forceinline__ bool wait(int stage) {
+        const uint32_t mine = ((1u << N) - 1) << stage, bulk = used & mine;
         bool ok = true;
-        if ((used >> stage) & 1) {
-            ok = ptx::mbar_wait_bounded(bars + 8 * stage, (phases >> stage) & 1, limit);
-            phases ^= 1u << stage;
-        } else {
-            asm volatile("cp.async.wait_all;" ::: "memory");
-        }
+        if (bulk != mine) asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if ((bulk >> (stage + i)) & 1) ok = ok && ptx::mbar_wait_bounded(bars + 8 * (stage + i), (phases >> (stage + i)) & 1, limit);
+        phases ^= bulk;
         if (__syncthreads_and(ok)) return true;
         if (threadIdx.x == 0) {
             atomicCAS(status, STATUS_OK, STATUS_FULL_WAIT_TIMEOUT);
-            if (!ptx::mbar_wait_bounded(bars + 8 * stage, ((phases >> stage) & 1) ^ 1, limit)) atomicCAS(status, STATUS_OK, STATUS_DRAIN_TIMEOUT);
+            for (int i = 0; i < N; i++)
+                if ((bulk >> (stage + i)) & 1 && !ptx::mbar_wait_bounded(bars + 8 * (stage + i), ((phases >> (stage + i)) & 1) ^ 1, limit)) atomicCAS(status, STATUS_OK, STATUS_DRAIN_TIMEOUT);
         }
         return false;
     }
 };
-__device__ __forceinline__ Stages make_stages(const DraftParams& p, uint64_t* bars) {
+__device__ __forceinline__ Stages make_stages(const DraftParams& p, uint64_t* bars, int n = G_STAGES) {
     Stages s;
     s.bars = (uint32_t)__cvta_generic_to_shared(bars);
     s.limit = p.wait_limit;
     s.status = p.status;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < G_STAGES; i++) ptx::mbar_init(s.bars + 8 * i, 1);
+        for (int i = 0; i < n; i++) ptx::mbar_init(s.bars + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_generic_kernel(const Draft
     }
 }
 
-// The same for at most 16 rows (chains, small trees): eight warps share the rows' work instead of the rows.  A warp multiplies an eighth of the
+// The same for at most 16 rows (chains, small trees; fp32 of heads of 64 or 128: 8): eight warps share the rows' work instead of the rows.  A warp multiplies an eighth of the
 // key's granules, the parts meet in shared memory, where every row has its warp for the softmax, and a warp has a quarter of the value's
 // columns, a lane each, for half of the tile's tokens.  Bound by the chain of a tile.  (With a warp's rows its own, few rows leave most warps
 // of a block idle and load one scheduler of the SM: one row of 2000 tokens, 32 fp32 heads of 128, 4 nodes: 62 us.)
@@ -582,16 +583,21 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_few_kernel(const DraftPara
     }
 }
 
-// fp32 with 17 rows and more, heads of 64 or 128: both products on the tensor cores (mma.sync, tf32), every operand as the sum of two tf32
-// numbers of 11 bits and three products of the four, which leaves out 2^-22 of a product: fp32 products on the CUDA cores ran at 9 TFLOP/s.
-// A block has 64 (32) rows; its warps are 4 (2) tiles of 16 rows times 2 (4) shares of every tile's 32 tokens, which meet at the end.
+// fp32 with 9 rows and more, heads of 64 or 128: both products on the tensor cores (mma.sync, tf32), every operand as the sum of two tf32
+// numbers of 11 bits and three products of the four, which leaves out 2^-22 of a product (fp32 products on the CUDA cores ran at 9 TFLOP/s).
+// A block has 64 (32) rows; its warps are 4 (2) tiles of 16 rows times 2 (4) shares of every tile's 32 tokens, which meet at the end.  Up to 16 rows:
+// eight shares of two tiles at a time, and no step of a tile waits for the other warps.
 // S = Q K^T: m16n8k8, A = queries, B = keys.  O += P V: the weights stay where the scores were, if an MMA's k index 2 j + i is token 2 j + i for
 // column j + 4 i: the values' rows are read in that order.
+// Operands are split by whole-number instructions: by cvt.rna, of which an SM does few a cycle, 8 rows of 1000 tokens with 120 query rows to each of 8 heads of
+// 64 took 98 us instead of 75.  One row of 4000 tokens, 32 heads of 128: 10 nodes 57 us, 8 nodes 57 (draft_few_kernel: 61 and 47); four rows of 288 and 9
+// nodes 20 (29).  What bounds few rows now are instructions (1150 a warp and 64 tokens, a third of them waited for) and one block an SM.
 struct Tf32Pair { uint32_t hi, lo; };
 __device__ __forceinline__ Tf32Pair split_tf32(float x) {
     Tf32Pair r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.hi) : "f"(x));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.lo) : "f"(x - __uint_as_float(r.hi)));
+    // rounded up from half: what is not a number may wrap to zero here, and stays what it is in lo
+    r.hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    r.lo = __float_as_uint(x - __uint_as_float(r.hi)) & 0xffffe000u;
     return r;
 }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -606,12 +612,14 @@ __device__ __forceinline__ void mma_pairs(float (&d)[4], const uint32_t (&ah)[4]
 }
 
 template <int D, int MT>  // head size; tiles of 16 rows
-__global__ void __launch_bounds__(G_THREADS, 2) draft_tf32_kernel(const __grid_constant__ DraftParams p, const GenericSizes z) {
+__global__ void __launch_bounds__(G_THREADS, MT == 1 && D == 128 ? 1 : 2) draft_tf32_kernel(const __grid_constant__ DraftParams p, const GenericSizes z) {
     extern __shared__ __align__(128) uint8_t raw[];
-    __shared__ uint64_t bars[G_STAGES];
-    constexpr int SHARES = G_WARPS / MT, NT = G_TOK / SHARES / 8, ROWS = 16 * MT, QP = D + 4, OP = D + 4;
-    float* const sq = reinterpret_cast<float*>(raw);     // [ROWS][QP]
-    uint8_t* const stages = raw + whole((int)sizeof(float) * ROWS * QP, 128);
+    constexpr int TILES = MT == 1 ? 2 : 1, STAGES = 2 * TILES;  // of 32 tokens, at a time
+    constexpr bool SPLIT = MT == 1;                             // queries are staged as two numbers
+    constexpr int SHARES = G_WARPS / MT, TILE_SHARES = SHARES / TILES, NT = G_TOK / TILE_SHARES / 8, ROWS = 16 * MT, QP = D + 4, OP = D + 4;
+    __shared__ uint64_t bars[STAGES];
+    float* const sq = reinterpret_cast<float*>(raw);     // [ROWS][QP], of pairs if SPLIT
+    uint8_t* const stages = raw + whole((int)sizeof(float) * ROWS * QP * (SPLIT ? 2 : 1), 128);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, oct = lane >> 2;
     const int G = p.geo.n_heads, group = p.group, H = G * group;
     const int kvh = blockIdx.x % G;
@@ -622,16 +630,38 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_tf32_kernel(const __grid_c
         if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
         return;
     }
-    const int n_rows = it.n_nodes * group, row0 = (warp % MT) * 16, tok0 = (warp / MT) * (G_TOK / SHARES);
+    const int n_rows = it.n_nodes * group, row0 = (warp % MT) * 16, mine = warp / MT / TILE_SHARES, tok0 = warp / MT % TILE_SHARES * (G_TOK / TILE_SHARES);
     const bool busy = row0 < n_rows;
     Walk<float> tiles(p, z, it, kvh, stages, make_int2(ic.x, ic.y));
-    Stages in = make_stages(p, bars);
-    Tile now = tiles.take();
+    Stages in = make_stages(p, bars, STAGES);
+    Tile now[TILES], after[TILES];
+#pragma unroll
+    for (int i = 0; i < TILES; i++) now[i] = tiles.take();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (now.n > 0) in.fetch(tiles, now, 0);
 #pragma unroll
-    for (int half = 0; half < ROWS / G_WARPS; half += 4) stage_queries<float, 4>(p, it, kvh, sq, QP, n_rows, ROWS, warp * (ROWS / G_WARPS) + half, 1);
+    for (int i = 0; i < TILES; i++)
+        if (now[i].n > 0) in.fetch(tiles, now[i], i);
+    if constexpr (SPLIT) {
+        float x[2][D / 32];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = min(warp + G_WARPS * i, n_rows - 1), at = r / group;
+            const float* from = static_cast<const float*>(p.q) + (int64_t)(it.node0 + at) * p.q_node + (int64_t)(kvh * group + r - at * group) * p.q_head;
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) x[i][c] = from[32 * c + lane];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                const Tf32Pair a = split_tf32(x[i][c]);
+                reinterpret_cast<uint2*>(sq)[(warp + G_WARPS * i) * QP + 32 * c + lane] = make_uint2(a.hi, a.lo);
+            }
+    } else {
+#pragma unroll
+        for (int half = 0; half < ROWS / G_WARPS; half += 4) stage_queries<float, 4>(p, it, kvh, sq, QP, n_rows, ROWS, warp * (ROWS / G_WARPS) + half, 1);
+    }
     float o[D / 8][4], m[2] = {G_NEG_BIG, G_NEG_BIG}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < D / 8; i++)
@@ -640,38 +670,62 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_tf32_kernel(const __grid_c
     const uint32_t* line[2];  // of rows oct and oct + 8
 #pragma unroll
     for (int h = 0; h < 2; h++) line[h] = p.seen + (int64_t)(it.node0 + min(row0 + oct + 8 * h, n_rows - 1) / group) * p.words;
-    for (int stage = 0; now.n > 0; stage ^= 1) {
-        if (!in.wait(stage)) return;  // nobody reads the tile before this one any more
-        const Tile after = tiles.take();
-        if (after.n > 0) in.fetch(tiles, after, stage ^ 1);
-        if (busy && tok0 < now.n) {
-            const uint8_t* const sk = stages + stage * z.stage();
+    for (int stage = 0; now[0].n > 0; stage ^= TILES) {
+        if (TILES == 2 && now[TILES - 1].n > 0) {
+            if (!in.wait<TILES>(stage)) return;
+        } else if (!in.wait(stage)) {
+            return;
+        }
+        // nobody reads the tiles before these any more
+#pragma unroll
+        for (int i = 0; i < TILES; i++) {
+            after[i] = tiles.take();
+            if (after[i].n > 0) in.fetch(tiles, after[i], (stage ^ TILES) + i);
+        }
+        const Tile at = TILES == 2 && mine ? now[TILES - 1] : now[0];
+        if (busy && tok0 < at.n) {
+            const uint8_t* const sk = stages + (stage + mine) * z.stage();
             const uint8_t* const sv = sk + G_TOK * z.k_bytes;
             uint32_t see[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                see[h] = now.n == 32 ? 0xffffffffu : (1u << now.n) - 1;
-                if (now.chunk < 0) see[h] &= __ldg(line[h] + now.first / 32);
+                see[h] = at.n == 32 ? 0xffffffffu : (1u << at.n) - 1;
+                if (at.chunk < 0) see[h] &= __ldg(line[h] + at.first / 32);
             }
-            float s[NT][4];
+            // few rows: one tile of scores a warp, so six sums of it, as a chain of products is what takes time
+            constexpr int SUMS = MT == 1 ? 6 : 1;
+            float s[NT][4], sums[SUMS][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int c = 0; c < SUMS; c++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) s[n][k] = 0.f;
-#pragma unroll 2
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) sums[c][n][k] = 0.f;
+#pragma unroll(MT == 1 && D == 128 ? 8 : 4)
             for (int ks = 0; ks < D / 8; ks++) {
                 uint32_t ah[4], al[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const Tf32Pair a = split_tf32(sq[(row0 + oct + 8 * (k & 1)) * QP + 8 * ks + quad + 4 * (k >> 1)]);
-                    ah[k] = a.hi;
-                    al[k] = a.lo;
+                    const int e = (row0 + oct + 8 * (k & 1)) * QP + 8 * ks + quad + 4 * (k >> 1);
+                    if constexpr (SPLIT) {
+                        const uint2 a = reinterpret_cast<const uint2*>(sq)[e];
+                        ah[k] = a.x;
+                        al[k] = a.y;
+                    } else {
+                        const Tf32Pair a = split_tf32(sq[e]);
+                        ah[k] = a.hi;
+                        al[k] = a.lo;
+                    }
                 }
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     const int t = tok0 + 8 * n + oct;
                     const float b0 = *reinterpret_cast<const float*>(sk + staged(t, 2 * ks, 0, 7) + 4 * quad), b1 = *reinterpret_cast<const float*>(sk + staged(t, 2 * ks + 1, 0, 7) + 4 * quad);
-                    mma_pairs(s[n], ah, al, split_tf32(b0), split_tf32(b1));
+                    const Tf32Pair p0 = split_tf32(b0), p1 = split_tf32(b1);
+                    const int c = SUMS == 6 ? 3 * (ks & 1) : 0;
+                    mma_tf32(sums[c][n], al, p0.hi, p1.hi);
+                    mma_tf32(sums[SUMS == 6 ? c + 1 : 0][n], ah, p0.lo, p1.lo);
+                    mma_tf32(sums[SUMS == 6 ? c + 2 : 0][n], ah, p0.hi, p1.hi);
                 }
             }
             float high[2] = {G_NEG_BIG, G_NEG_BIG};
@@ -679,6 +733,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_tf32_kernel(const __grid_c
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
+                    s[n][k] = SUMS == 6 ? ((sums[0][n][k] + sums[SUMS / 2][n][k]) + (sums[SUMS / 6][n][k] + sums[SUMS * 4 / 6][n][k])) + (sums[SUMS / 3][n][k] + sums[SUMS * 5 / 6][n][k]) : sums[0][n][k];
                     s[n][k] = (see[k >> 1] >> (tok0 + 8 * n + 2 * quad + (k & 1))) & 1 ? s[n][k] * p.scale_log2 : -INFINITY;
                     high[k >> 1] = fmaxf(high[k >> 1], s[n][k]);
                 }
@@ -716,7 +771,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_tf32_kernel(const __grid_c
                 }
                 // values behind the tile's tokens are anything: zero
                 const int t = tok0 + 8 * n + 2 * quad;
-                const bool on0 = t < now.n, on1 = t + 1 < now.n;
+                const bool on0 = t < at.n, on1 = t + 1 < at.n;
 #pragma unroll
                 for (int i = 0; i < D / 8; i++) {
                     const int c = 8 * i + oct;
@@ -725,7 +780,8 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_tf32_kernel(const __grid_c
                 }
             }
         }
-        now = after;
+#pragma unroll
+        for (int i = 0; i < TILES; i++) now[i] = after[i];
     }
     // ---- the shares of a row meet
     __syncthreads();
@@ -780,6 +836,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_tf32_kernel(const __grid_c
 }
 
 constexpr int MOST_SHARED = 232448;  // of a CTA
+bool tf32_serves(int block_rows, int dk, int dv, int esize) { return esize == 4 && block_rows > 8 && dk == dv && (dk == 64 || dk == 128); }
 
 template <typename T>
 cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t stream) {
@@ -793,8 +850,10 @@ cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t st
     auto few = [&](auto* k, int r) { return go(k, G_THREADS, (size_t)r * (z.q_floats + (G_WARPS + 1) * G_TOK + 3)); };
     auto many = [&](auto* k, int rw) { return go(k, G_THREADS, (size_t)G_WARPS * rw * (z.q_floats + G_TOK)); };
     if constexpr (sizeof(T) == 4) {
-        if (block_rows > 16 && p.d_key == p.d_value && (p.d_key == 64 || p.d_key == 128) && p.geo.swz && p.geo.v_swz) {
+        if (tf32_serves(block_rows, p.d_key, p.d_value, 4) && p.geo.swz && p.geo.v_swz) {
             auto tf32 = [&](auto* k, int rows, int d) { return go(k, G_THREADS, std::max((size_t)rows * (d + 4), (size_t)G_WARPS * 16 * (d + 6) - G_STAGES * z.stage() / 4)); };
+            const size_t few_floats = 2 * 16 * (p.d_key + 4) + 2 * z.stage() / 4;  // two stages more
+            if (block_rows <= 16) return p.d_key == 64 ? go(&draft_tf32_kernel<64, 1>, G_THREADS, few_floats) : go(&draft_tf32_kernel<128, 1>, G_THREADS, few_floats);
             if (p.d_key == 64) return block_rows <= 32 ? tf32(&draft_tf32_kernel<64, 2>, 32, 64) : tf32(&draft_tf32_kernel<64, 4>, 64, 64);
             return block_rows <= 32 ? tf32(&draft_tf32_kernel<128, 2>, 32, 128) : tf32(&draft_tf32_kernel<128, 4>, 64, 128);
         }
@@ -946,6 +1005,7 @@ __global__ void __launch_bounds__(32) accept_draft_kernel(const AcceptParams p) 
 
 int draft_generic_ctas(int block_rows, int dk, int dv, int esize) {
     const GenericSizes z = generic_sizes(dk, dv, esize);
+    if (block_rows <= 16 && tf32_serves(block_rows, dk, dv, esize)) return dk == 64 ? 2 * B200_SMS : B200_SMS;
     const int rows = sizeof(float) * block_rows * (z.q_floats + (block_rows <= 16 ? (G_WARPS + 1) * G_TOK + 3 : G_TOK));
     return B200_SMS * std::max(1, std::min(2, MOST_SHARED / (rows + G_STAGES * z.stage() + 1024 + 128)));
 }
