@@ -14,6 +14,12 @@
 // Warp roles: 0-3 softmax and epilogue, 4 TMA producer over a ring of four tile slots, 5 TMEM and the MMA issue, 6 the next piece
 // of work (a CTA takes over pieces that have not been launched yet: cluster launch control).  Two CTAs share an SM.
 //
+// What bounds it: with few rows to a tile HBM, and the ends of a piece (queries, first scores, last values, epilogue: 4.2 us together, of which
+// the other CTA of the SM hides a part): 32 rows of 2048 shared and 512 own tokens, 32 heads, 13 nodes 84 us, 0.57 of the copy rate; 64 rows of up to 1024
+// tokens, 8 heads of 4, 24 nodes 49 us (0.70).  With full blocks the tensor pipe, 384 cycles of scores (their operands' way from shared memory) and
+// 512 of two products with V of some 1170 a tile: 8 rows of up to 16000, 8 heads of 8, 63 nodes 210 us.  One product with V would
+// take 256 less, but rounds weights to 8 bits.
+//
 // A row of which an element comes out as not finite is computed once more on CUDA cores: a value that is infinite may be one that the row does
 // not see (0 * infinity), and hi + lo parts of a weight times infinity are not its product.
 //
