@@ -45,14 +45,17 @@ constexpr int L_ROWS = 3;                 // rows that may be at hand: one is be
 constexpr int F_THREADS = 128, F_WARPS = F_THREADS / 32;
 constexpr float L_RESCALE = 8.f;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float L_HIGHEST = 0x1p30f;      // references from here on leave more of their rounding in the exponents than 2^y can hold
 constexpr int NO_ID = 0x7fffffff;
 
-// Excluded logits count as this finite value, so that 0 * y stays 0.  A power of two: its product with log2 e is exact, so a lane that has met
-// nothing else gets y = 0 (rounded, the rest of 10^30 would be 10^22)
-template <typename T> __device__ __forceinline__ constexpr float floor_of() { return -0x1p100f; }
+// Excluded and masked logits count as this finite value at least, so that 0 * y stays 0.  A reference is a rounded product, high * log2 e, and what its
+// rounding leaves stands in the exponents of the lane: half a step of the product, 64 at 2^30, which 2^y can hold (next to -10^10 512, which
+// it cannot: a lane that had met nothing but such masks made its whole row NaN).  A logit above the floor is above it by 64 (fp32) at least, so e^-64
+// of it is all that a lower one may count too much.
+template <typename T> __device__ __forceinline__ constexpr float floor_of() { return -0x1p30f; }
 template <> __device__ __forceinline__ constexpr float floor_of<__half>() { return -65504.f; }
 // The least threshold: the bf16 (fp16) number above it
-template <typename T> __device__ __forceinline__ constexpr float least_of() { return -0x1.fep99f; }
+template <typename T> __device__ __forceinline__ constexpr float least_of() { return -0x1.fep29f; }
 template <> __device__ __forceinline__ constexpr float least_of<__half>() { return -65472.f; }
 
 // A vector of logits, 16 bytes
@@ -93,7 +96,7 @@ template <typename T> struct Vec {
             return __float_as_uint(fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])), fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3]))));
         } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(0xf180f180u));
+            for (int i = 0; i < 4; i++) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(0xce80ce80u));
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(0xfbfffbffu));
@@ -297,7 +300,7 @@ template <typename T, bool TOP, int THREADS> __device__ __forceinline__ void fin
         float log_l = logf(st.l), lse_m = st.m * LN2, entropy = log_l - LN2 * (st.a / st.l);
         // Nothing above the floor, or nothing that can be scaled: a row of lowest values (uniform over them), of nothing but excluded tokens, of
         // the largest values, of infinity.  Walked again as the formulas say.
-        if (st.m <= floor_of<T>() * LOG2E || st.m >= 1.0e37f) {
+        if (st.m <= floor_of<T>() * LOG2E || st.m >= L_HIGHEST) {
             float high = -INFINITY, sum = 0.f, weighted = 0.f;
             bool nan = false;
             for (int i = lane; i < p.vocab; i += 32) {

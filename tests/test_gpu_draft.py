@@ -407,6 +407,45 @@ def test_log_probs_of_excluded_tokens(dtype):
     check_log_probs(y, 3)
 
 
+def check_log_probs_closely(logits, top, more=0.0):
+    """What only the differences of a row's logits allow, whatever their size.  The sum of exponentials: a lane adds up to vocab / 256 pairs and some 32
+    partial sums, each addition off by 2^-24; a term by 2^-22 (the exponential) and by its argument's rounding, 2^-24 of some 24 log2
+    units: 2^-20 together.  That is the log's error, and the result is rounded to fp32.  The entropy weighs logs of up to some 32 with such terms."""
+    from chunk_attn import ops
+    n, vocab = logits.shape
+    tokens = torch.arange(n, dtype=torch.int32, device=DEV) % vocab
+    got = ops.token_log_probs(logits, tokens, None, top)
+    want = D.log_probs(logits, tokens, torch.arange(n, device=DEV), top)
+    assert torch.equal(got[3].long(), want[3]), "top tokens differ"
+    close = 2.0 ** -24 * (vocab / 256 + 32) + 2.0 ** -20 + more
+    for name, a, b, tol in (("log_probs", got[0], want[0], close), ("entropy", got[1], want[1], 32 * close), ("top", got[2], want[2], close)):
+        assert torch.isfinite(a).all(), name
+        err = (a.double() - b).abs()
+        assert (err <= tol + 2.0 ** -23 * b.abs()).all(), "%s: off by %g" % (name, (err - 2.0 ** -23 * b.abs()).max().item())
+    return got
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("n,vocab,kept", [(3, 20000, 300), (700, 8000, 300), (2, 3001, 2), (40, 40000, 5)])
+def test_log_probs_of_masked_tokens(dtype, n, vocab, kept):
+    """Finite masks of any size, over so many tokens that threads meet nothing else: what is left has the distribution.  Rows of nothing but such logits,
+    and of such large ones, too."""
+    for mask in (-1e4, -65504.0, -1e9, -2.0 ** 30, -2e9, -1e10, -1e15, -1e20, -1e30, -1e35, -3e38):
+        if dtype == F16 and mask < -65504:
+            continue
+        x = torch.randn(n, vocab, device=DEV, generator=torch.Generator(DEV).manual_seed(6)) * 3
+        x[:, kept:] = mask
+        got = check_log_probs_closely(x.to(dtype), 5, more=2.0 ** -21 * 16)  # logits of up to 16
+        if kept < 5:  # the masked ones follow by their ids
+            assert got[3][:, kept:].tolist() == [list(range(kept, 5))] * n
+    for high in (-1e30, -1e10, 1e9, 1e10, 1e20, 1e30):
+        if dtype == F16:
+            continue
+        x = torch.full((n, vocab), high, device=DEV)
+        x[:, ::3] *= 1.25 if high < 0 else 0.75
+        check_log_probs_closely(x.to(dtype), 5)
+
+
 def test_log_probs_far_from_zero():
     """Large logits: only their differences count."""
     g = torch.Generator(DEV).manual_seed(4)
