@@ -44,7 +44,7 @@ constexpr int L_GROUPS = 64;              // of threads, at most
 constexpr int L_ROWS = 3;                 // rows that may be at hand: one is begun, one finished, one cleared
 constexpr int F_THREADS = 128, F_WARPS = F_THREADS / 32;
 constexpr float L_RESCALE = 8.f;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr float L_HIGHEST = 0x1p30f;      // references from here on leave more of their rounding in the exponents than 2^y can hold
 constexpr int NO_ID = 0x7fffffff;
 
@@ -202,7 +202,7 @@ struct Shared {
     int n_hits[L_ROWS];
     int n_found;
     float limit;
-    float2 lse;
+    double2 lse;
     union {
         uint32_t hits[L_ROWS][L_HITS];
         struct {                    // a row that a cluster finishes is the only one
@@ -293,11 +293,23 @@ template <typename T> __device__ __noinline__ Best best_slowly(const T* x, int l
     return best;
 }
 
+// ln of a sum of terms, the largest of which is 2^-8 at least: the exponent's part exact, the rest below ln 2
+__device__ __forceinline__ double log_of(float sum) {
+    if (!(sum < INFINITY)) return NAN;
+    const int e = ((__float_as_int(sum) >> 23) & 255) - 127;
+    return e * 0.69314718055994530942 + (double)logf(__int_as_float(__float_as_int(sum) - (e << 23)));
+}
+// Differences of a logit and what its row's sum says are of 64 bits: either may be large and both rounded, where only their difference counts.
+__device__ __forceinline__ float log_prob(float x, double2 lse) { return (float)(((double)x - lse.x) - lse.y); }
+
 // What is known of a row: results, and the log probabilities of tokens that are asked of it.  A whole CTA; st, best: warp 0's.
-template <typename T, bool TOP, int THREADS> __device__ __forceinline__ void finish_row(const LogProbsParams& p, float2& shared_lse, const T* x, int row, Stat st, Best best) {
+template <typename T, bool TOP, int THREADS> __device__ __forceinline__ void finish_row(const LogProbsParams& p, double2& shared_lse, const T* x, int row, Stat st, Best best) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
-        float log_l = logf(st.l), lse_m = st.m * LN2, entropy = log_l - LN2 * (st.a / st.l);
+        // The sum is that of 2^(LOG2E x - m), LOG2E being the fp32 number: m / LOG2E is the reference in the logits' units, and the rounding of neither product nor
+        // constant is left in it (m ln 2 in fp32 was 4e-5 off next to 1000, 5e-3 next to 10^5)
+        double2 lse = {(double)st.m * (1.0 / (double)LOG2E), log_of(st.l)};
+        float entropy = (float)(lse.y - (double)(st.a / st.l) * (1.0 / (double)LOG2E));
         // Nothing above the floor, or nothing that can be scaled: a row of lowest values (uniform over them), of nothing but excluded tokens, of
         // the largest values, of infinity.  Walked again as the formulas say.
         if (st.m <= floor_of<T>() * LOG2E || st.m >= L_HIGHEST) {
@@ -316,27 +328,26 @@ template <typename T, bool TOP, int THREADS> __device__ __forceinline__ void fin
             }
             sum = warp_sum(sum);
             weighted = warp_sum(weighted);
-            log_l = logf(sum);
-            lse_m = high;
-            entropy = log_l - weighted / sum;
-            if (__any_sync(0xffffffffu, nan) || high == -INFINITY) log_l = lse_m = entropy = NAN;
+            lse = {(double)high, (double)logf(sum)};
+            entropy = (float)(lse.y - (double)(weighted / sum));
+            if (__any_sync(0xffffffffu, nan) || high == -INFINITY) lse.x = lse.y = entropy = NAN;
         }
         if (lane == 0) {
             p.entropy[row] = entropy;
-            shared_lse = make_float2(lse_m, log_l);
-            if (!p.tokens_here) p.lse[row] = make_float2(lse_m, log_l);
+            shared_lse = lse;
+            if (!p.tokens_here) p.lse[row] = lse;
         }
         if (TOP && lane < p.top) {
             p.top_ids[(int64_t)row * p.top + lane] = best.i;
-            p.top_log_probs[(int64_t)row * p.top + lane] = (best.v - lse_m) - log_l;
+            p.top_log_probs[(int64_t)row * p.top + lane] = log_prob(best.v, lse);
         }
     }
     if (p.tokens_here && p.n_tokens > 0) {
         __syncthreads();
-        const float2 lse = shared_lse;
+        const double2 lse = shared_lse;
         auto one = [&](int i) {
             const int token = p.tokens[i];
-            p.log_probs[i] = token == -1 ? 0.f : (token >= 0 && token < p.vocab ? (to_f32(x[token]) - lse.x) - lse.y : NAN);
+            p.log_probs[i] = token == -1 ? 0.f : (token >= 0 && token < p.vocab ? log_prob(to_f32(x[token]), lse) : NAN);
         };
         if (!p.rows) {
             if (threadIdx.x == 0) one(row);
@@ -663,7 +674,7 @@ template <typename T, bool TOP>
 __global__ void __launch_bounds__(F_THREADS) finish_rows_kernel(const LogProbsParams p, int n_ctas) {
     __shared__ Best found[L_FOUND], list[F_WARPS][32];
     __shared__ int n_found;
-    __shared__ float2 lse;
+    __shared__ double2 lse;
     const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, k = max(1, p.top);
     // the stretches of CTAs b0 .. b1: the one in which the row begins and those that begin inside it
     const int64_t row_begin = (int64_t)row * p.turns;
@@ -733,8 +744,8 @@ __global__ void __launch_bounds__(128) given_tokens_kernel(const LogProbsParams 
     const int row = p.rows ? p.rows[i] : i, token = p.tokens[i];
     float lp = NAN;
     if (row >= 0 && row < p.n_rows) {
-        const float2 lse = p.lse[row];
-        if (token >= 0 && token < p.vocab) lp = (to_f32(static_cast<const T*>(p.logits)[(int64_t)row * p.row_stride + token]) - lse.x) - lse.y;
+        const double2 lse = p.lse[row];
+        if (token >= 0 && token < p.vocab) lp = log_prob(to_f32(static_cast<const T*>(p.logits)[(int64_t)row * p.row_stride + token]), lse);
         if (token == -1) lp = 0.f;
     }
     p.log_probs[i] = lp;

@@ -28,7 +28,7 @@ struct LogProbsParams {
     float* top_log_probs;    // [n_rows, top]
     int32_t* top_ids;
     LogProbsPart* parts;     // [n_rows + log_probs_ctas()], when stretches are handed out
-    float2* lse;             // [n_rows]: maximum, log of the sum relative to it
+    double2* lse;            // [n_rows]: a reference, log of the sum relative to it
     bool tokens_here;        // the rows' CTAs look the tokens up, else a kernel behind them does
 #if defined(__CUDACC__)
     __device__ __forceinline__ int64_t begin(int b) const { return b * each + min(b, more); }

@@ -454,6 +454,21 @@ def test_log_probs_far_from_zero():
     check_log_probs(torch.randn(4, 6000, device=DEV, generator=g) * 1e-6 - 50, 4)
 
 
+@pytest.mark.parametrize("n,vocab,top", [(64, 6000, 5), (1, 32000, 20), (700, 9001, 3), (3, 100, 0)])
+def test_log_probs_do_not_go_by_the_size_of_logits(n, vocab, top):
+    """Rows far from zero, and rows with a token that takes nearly all: the error is that of rows around zero."""
+    x = torch.randn(n, vocab, device=DEV, generator=torch.Generator(DEV).manual_seed(7)) * 2.5
+    for offset in (0.0, 30.0, -30.0, 300.0, -1000.0, 1e4, 1e5, -1e6, 2.0 ** 25, 5e8):
+        check_log_probs_closely(x + offset, top)
+        y = x + offset
+        y[:, 0] = offset + max(40.0, abs(offset) * 2.0 ** -20)
+        check_log_probs_closely(y, top)
+    check_log_probs_closely(x * 300, top)
+    for offset in (30.0, 300.0):  # 16-bit steps of 0.25 (fp16) and 2 (bf16)
+        check_log_probs_closely((x + offset).half(), top)
+        check_log_probs_closely((x + offset).bfloat16(), top)
+
+
 def test_log_probs_of_named_tokens():
     from chunk_attn import ops
     x = torch.randn(4, 100, device=DEV)
