@@ -1924,6 +1924,7 @@ int ca_token_log_probs(const ca_log_probs_args* a, ca_stream stream) {
     if (a->row_stride < 0) return fail(CA_ERR_INVALID, "token_log_probs: negative stride");
     if (a->n_rows > 0 && (!a->logits || !a->entropy || !a->scratch)) return fail(CA_ERR_INVALID, "token_log_probs: null operand");
     if (a->n_tokens > 0 && (!a->tokens || !a->log_probs)) return fail(CA_ERR_INVALID, "token_log_probs: null operand");
+    if (!a->rows && a->n_tokens > 0 && a->n_tokens != a->n_rows) return fail(CA_ERR_INVALID, "token_log_probs: without rows, one token per row is required");
     if (a->n_rows > 0 && a->top > 0 && (!a->top_ids || !a->top_log_probs)) return fail(CA_ERR_INVALID, "token_log_probs: null operand");
     if (reinterpret_cast<uintptr_t>(a->logits) % shaped_esize_of(a->dtype) || reinterpret_cast<uintptr_t>(a->scratch) % 16)
         return fail(CA_ERR_INVALID, "token_log_probs: logits must be aligned to their type, scratch to 16 bytes");

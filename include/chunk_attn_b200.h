@@ -705,7 +705,7 @@ typedef struct ca_accept_args {
 CA_API int ca_accept_draft(const ca_accept_args* args, ca_stream stream);
 
 /* Log probabilities from logits [n_rows, vocab] (any type, rows row_stride elements apart): with lse = log sum exp of a row,
- * log_probs[i] = logits[rows[i]][tokens[i]] - lse (rows NULL: i; token -1: 0; other ids or rows out of range: NaN),
+ * log_probs[i] = logits[rows[i]][tokens[i]] - lse (rows NULL: i, and n_tokens is n_rows or 0; token -1: 0; other ids or rows out of range: NaN),
  * entropy[r] = lse - sum p x, and the top best tokens of a row by value, of equal ones those with the lowest ids:
  * top_ids, top_log_probs [n_rows, top].  Excluded tokens (-infinity) have probability 0.  A row that holds a NaN, +infinity or nothing
  * but -infinity has no distribution: its numbers are NaN (top_ids counts NaN as -infinity).  scratch: ca_log_probs_scratch bytes,

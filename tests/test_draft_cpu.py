@@ -175,3 +175,11 @@ def test_log_probs_refuse_at_the_c_entry():
     assert cabi.lib.ca_token_log_probs(None, None) != cabi.CA_OK
     for bad in ((-1, 10, cabi.CA_DTYPE_F32, 1), (1, 0, cabi.CA_DTYPE_F32, 1), (1, 10, 9, 1), (1, 10, cabi.CA_DTYPE_F32, 33)):
         assert cabi.lib.ca_log_probs_scratch(*bad) < 0
+
+
+def test_log_probs_without_rows_take_a_token_for_every_row():
+    """The kernels give every row its token, so another number of them would be read and written behind the arrays' ends, or left unwritten."""
+    ok = {n: 4096 for n, t in LogProbsArgs._fields_ if t is C.c_void_p}
+    ok.update(row_stride=100, n_rows=4, vocab=100, dtype=cabi.CA_DTYPE_F32, n_tokens=4, top=3, rows=0)
+    for change in ({"n_tokens": 3}, {"n_tokens": 5}, {"n_rows": 0}, {"n_tokens": 1, "top": 0}):
+        refused(cabi.lib.ca_token_log_probs, LogProbsArgs(**dict(ok, **change)), "one token per row")
