@@ -1852,6 +1852,7 @@ int ca_draft_attention(ca_context* c, const ca_draft_args* a, ca_stream stream_)
     p.status = c->status;
     p.wait_limit = c->opt_wait_limit;
     p.dependent = c->opt_pdl;
+    p.settled = a->settled != 0;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (a->info->block_rows == ca::DRAFT_TC_ROWS) {
         if (!draft_on_tensor_cores(c)) return fail(CA_ERR_STATE, "drafted tokens: the work list was made for other kernels");

@@ -45,7 +45,7 @@ template <typename T> struct Walk {
     uint8_t* const stages;
     int j = 0, t0 = 0, d0 = 0, chunk = -1, in_chunk = 0;
     int2 next;  // chunk j's pair, asked for a chunk ahead
-    __device__ __forceinline__ int2 entry(int i) const { return i < it.n_tiles ? __ldg(reinterpret_cast<const int2*>(p.tiles) + it.list + i) : make_int2(-1, 0); }
+    __device__ __forceinline__ int2 entry(int i) const { return i < it.n_tiles ? list_load(reinterpret_cast<const int2*>(p.tiles) + it.list + i) : make_int2(-1, 0); }
     __device__ __forceinline__ Walk(const DraftParams& p, const GenericSizes& z, const DraftItem& it, int kvh, uint8_t* stages, int2 first) : p(p), z(z), it(it), kvh(kvh), stages(stages), next(first) {}
     __device__ __forceinline__ Tile take() {
         while (j < it.n_tiles) {
@@ -205,8 +205,9 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_generic_kernel(const Draft
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = p.geo.n_heads, group = p.group, H = G * group;
     const int kvh = blockIdx.x % G;
-    const int4 ia = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G)), ib = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 1),
-               ic = __ldg(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 2);
+    draft_lists_wait(p);
+    const int4 ia = list_load(reinterpret_cast<const int4*>(p.items + blockIdx.x / G)), ib = list_load(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 1),
+               ic = list_load(reinterpret_cast<const int4*>(p.items + blockIdx.x / G) + 2);
     const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w, {}};
     if (!draft_item_ok(p, ia, ib, G_WARPS * RW)) {
         if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_generic_kernel(const Draft
         for (int c = 0; c < COLS * 4; c++) o[r][c] = 0.f;
     }
     Stages in = make_stages(p, bars);
-    // the work list is old; what it names is the kernels' before
+    // what the work list names is the kernels' before
     Tile now = tiles.take();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_generic_kernel(const Draft
 #pragma unroll
             for (int r = 0; r < RW; r++) {
                 line[r] = now.n == 32 ? 0xffffffffu : (1u << now.n) - 1;
-                if (drafted) line[r] &= __ldg(p.seen + (int64_t)(it.node0 + min(row0 + r, n_rows - 1) / group) * p.words + now.first / 32);
+                if (drafted) line[r] &= list_load(p.seen + (int64_t)(it.node0 + min(row0 + r, n_rows - 1) / group) * p.words + now.first / 32);
                 s[r] = (line[r] >> lane) & 1 ? s[r] * p.scale_log2 : -INFINITY;
                 high[r] = s[r];
             }
@@ -389,8 +390,9 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_few_kernel(const DraftPara
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = p.geo.n_heads, group = p.group, H = G * group;
     const int kvh = blockIdx.x % G;
+    draft_lists_wait(p);
     const int4* const item = reinterpret_cast<const int4*>(p.items + blockIdx.x / G);
-    const int4 ia = __ldg(item), ib = __ldg(item + 1), ic = __ldg(item + 2);
+    const int4 ia = list_load(item), ib = list_load(item + 1), ic = list_load(item + 2);
     const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w, {}};
     if (!draft_item_ok(p, ia, ib, R)) {
         if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_few_kernel(const DraftPara
             for (int i = 0; i < MINE; i++) {
                 const int r = min(warp + G_WARPS * i, R - 1);
                 uint32_t line = there;
-                if (drafted) line &= __ldg(p.seen + (int64_t)(it.node0 + min(r, n_rows - 1) / group) * p.words + now.first / 32);
+                if (drafted) line &= list_load(p.seen + (int64_t)(it.node0 + min(r, n_rows - 1) / group) * p.words + now.first / 32);
                 see[i] = (line >> lane) & 1;
                 float x = 0.f;
 #pragma unroll
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(G_THREADS, 2) draft_few_kernel(const DraftPara
             int node = it.node0, in_group = 0;
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                line[r] = drafted && r < n_rows ? there & __ldg(p.seen + (int64_t)node * p.words + now.first / 32) : there;
+                line[r] = drafted && r < n_rows ? there & list_load(p.seen + (int64_t)node * p.words + now.first / 32) : there;
                 if (++in_group == group) {
                     in_group = 0;
                     node++;
@@ -624,8 +626,9 @@ __global__ void __launch_bounds__(G_THREADS, MT == 1 && D == 128 ? 1 : 2) draft_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, oct = lane >> 2;
     const int G = p.geo.n_heads, group = p.group, H = G * group;
     const int kvh = blockIdx.x % G;
+    draft_lists_wait(p);
     const int4* const item = reinterpret_cast<const int4*>(p.items + blockIdx.x / G);
-    const int4 ia = __ldg(item), ib = __ldg(item + 1), ic = __ldg(item + 2);
+    const int4 ia = list_load(item), ib = list_load(item + 1), ic = list_load(item + 2);
     const DraftItem it = {ia.x, ia.y, ia.z, ia.w, ib.x, ib.y, ib.z, ib.w, {}};
     if (!draft_item_ok(p, ia, ib, ROWS)) {
         if (tid == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
@@ -691,7 +694,7 @@ __global__ void __launch_bounds__(G_THREADS, MT == 1 && D == 128 ? 1 : 2) draft_
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 see[h] = at.n == 32 ? 0xffffffffu : (1u << at.n) - 1;
-                if (at.chunk < 0) see[h] &= __ldg(line[h] + at.first / 32);
+                if (at.chunk < 0) see[h] &= list_load(line[h] + at.first / 32);
             }
             // few rows: one tile of scores a warp, so six sums of it, as a chain of products is what takes time
             constexpr int SUMS = MT == 1 ? 6 : 1;
@@ -876,14 +879,15 @@ cudaError_t launch_generic(const DraftParams& p, int block_rows, cudaStream_t st
 }
 
 // ---- combination: a warp for every (node, query head) that several items serve ---------------------------------------------------
-// Its latency is all there is to it: which partial results a node has is read while the kernel before still runs (the work list has long been
-// there), and their rows are requested together with the maxima and sums, eight at a time.
+// Its latency is all there is to it: which partial results a node has is read while the kernel before still runs, where the work list has long been
+// there, and their rows are requested together with the maxima and sums, eight at a time.
 template <typename T, int COLS>
 __global__ void __launch_bounds__(128) draft_merge_kernel(const DraftParams p) {
     constexpr int BATCH = COLS == 1 ? 8 : 4;
     const int H = p.geo.n_heads * p.group, lane = threadIdx.x & 31;
     const int pair = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (pair >= p.n_merge * H) return;
+    draft_lists_wait(p);
     const int i = pair / H, head = pair % H;
     const int node = p.merge_nodes[i], b = p.merge_off[i], n = p.merge_off[i + 1] - b;
     int slot = lane < n ? p.merge_slots[b + lane] : 0;

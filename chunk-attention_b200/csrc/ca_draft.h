@@ -81,7 +81,14 @@ struct DraftParams {
     int* status;
     long long wait_limit;
     int dependent;             // CA_OPT_DEPENDENT_LAUNCH
+    bool settled;              // the work list and seen may be read while the kernel before runs
 };
+// First of all in every kernel: unless nothing that still runs writes the work list and seen, wait for the kernels before
+__device__ __forceinline__ void draft_lists_wait(const DraftParams& p) {
+    if (!p.settled) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// What the lists hold may have been written after the kernel began, before its wait: plain loads, which stay behind it
+template <typename T> __device__ __forceinline__ T list_load(const T* p) { return *p; }
 // nothing in a work list is trusted
 __device__ __forceinline__ bool draft_item_ok(const DraftParams& p, int4 a, int4 b, int block_rows) {
     return a.x >= 0 && a.y > 0 && a.x + a.y <= p.n_nodes && a.y * p.group <= block_rows && a.z >= 0 && a.w >= 0 && a.z + a.w <= p.n_list &&

@@ -147,9 +147,10 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
     __syncthreads();
     tc_fence_after_thread_sync();
     const uint32_t tmem_base = *tmem_slot;
-    // with tensor memory in hand: a kernel behind this one may allocate, too.  Only the producer waits for the kernels before: the work list and the
-    // trees' bits have long been there (they came by copies, which no kernel overtakes), and what is stored follows from what is loaded.
+    // with tensor memory in hand: a kernel behind this one may allocate, too.  Where the work list and the trees' bits have long been there (they came by
+    // copies, which no kernel overtakes), only the producer waits for the kernels before: what is stored follows from what is loaded.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    draft_lists_wait(p);
     // a wait of a single thread: false, with the code recorded, when the limit ran out
     auto wait = [&](uint32_t bar, int parity, int code) {
         if (mbar_wait_bounded(bar, parity, p.wait_limit)) return true;
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                 Work w{};
                 if (item >= 0) {
                     const int4* it = reinterpret_cast<const int4*>(p.items + item / G);
-                    const int4 a = __ldg(it), b = __ldg(it + 1), c = __ldg(it + 2), d = __ldg(it + 3);
+                    const int4 a = list_load(it), b = list_load(it + 1), c = list_load(it + 2), d = list_load(it + 3);
                     w.head[0] = make_int2(c.x, c.y);
                     w.head[1] = make_int2(c.z, c.w);
                     w.head[2] = make_int2(d.x, d.y);
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
                     queue[0] = queue[1];
                     queue[1] = queue[2];
                     queue[2] = queue[3];
-                    queue[3] = j + 4 < w.n_context ? __ldg(tiles + j + 4) : make_int2(0, 0);
+                    queue[3] = j + 4 < w.n_context ? list_load(tiles + j + 4) : make_int2(0, 0);
                     if (j < w.n_context && (tile.x < 0 || tile.x >= p.max_chunks || tile.y <= 0 || tile.y > A_TOK)) {
                         report(p.status, STATUS_BAD_WORK_LIST);  // keep the pipeline moving on a chunk that exists
                         tile = make_int2(0, A_TOK);
@@ -349,10 +350,10 @@ __global__ void __launch_bounds__(A_THREADS, 2) draft_attn_kernel(const __grid_c
             for (int j = 0; j < w.n_tiles; j++, t++) {
                 const int b = t & 1;
                 const bool drafted = j >= w.n_context;
-                const int stored = drafted ? 0 : (j == 0 ? w.head[0].y : __ldg(p.tiles + 2 * (w.list + j) + 1));
+                const int stored = drafted ? 0 : (j == 0 ? w.head[0].y : list_load(p.tiles + 2 * (w.list + j) + 1));
                 const int filled = drafted ? min(A_TOK, w.n_drafted - (j - w.n_context) * A_TOK) : max(0, min(A_TOK, stored));
                 uint2 see = make_uint2(0u, 0u);
-                if (drafted) see = __ldg(line + (j - w.n_context));
+                if (drafted) see = list_load(line + (j - w.n_context));
                 if (!(live = wait_all(s_full + 8 * b, (t >> 1) & 1))) break;
                 tc_fence_after_thread_sync();
                 float alpha = 1.f;

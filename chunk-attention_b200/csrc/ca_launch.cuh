@@ -11,8 +11,9 @@ namespace ca {
 // CA_OPT_DEPENDENT_LAUNCH, as launches carry it
 constexpr int DEPENDENT_MERGE = 1, DEPENDENT_ATTENTION = 2;
 
-// dependent: the kernel is set up while the one ahead drains; it executes griddepcontrol.wait before it touches global memory.  Where the
-// stream or the driver refuses that (or CA_DISABLE_PDL is set), an ordinary launch.  cluster: CTAs of a cluster, along x.
+// dependent: the kernel is set up while the one ahead drains; it executes griddepcontrol.wait before it touches global memory that a kernel may have
+// written (work lists that came by copies it may read before).  Where the stream or the driver refuses that (or CA_DISABLE_PDL is
+// set), an ordinary launch.  cluster: CTAs of a cluster, along x.
 template <typename... P, typename... A>
 cudaError_t launch_kernel(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, bool dependent, cudaStream_t stream, const A&... args) {
     static const bool disabled = std::getenv("CA_DISABLE_PDL") != nullptr;

@@ -642,6 +642,7 @@ torch::Tensor Attention::forward_draft(torch::Tensor q, torch::Tensor k, torch::
     a.words = draft.words();
     a.work = draft_->device.use();
     a.info = &draft_->info;
+    a.settled = 1;  // both came by copies, which use() has waited for
     if (capturing(options_.device())) captured_.push_back(draft_->device.tensor());  // a replay reads it, whatever the tree has become
     torch::Tensor scratch;
     const int64_t floats = ca_draft_partial_floats(ctx_, a.info);

@@ -128,8 +128,8 @@ CA_API int ca_context_create_shaped(ca_context** out, int device, const ca_head_
 #define CA_OPT_TRACE 4
 /* programmatic dependent launches: bit 0, the merge kernel is set up while the attention kernel
  * drains; bit 1, the attention kernel is set up while the kernel before it in the stream finishes
- * (it waits for that kernel's completion before it touches global memory; the item kernel of grouped heads
- * is always launched in the ordinary way).  Default 3. */
+ * (it waits for that kernel's completion before it touches global memory, but for work lists that a refresh or,
+ * as the caller says, a copy has brought; the item kernel of grouped heads is always launched in the ordinary way).  Default 3. */
 #define CA_OPT_DEPENDENT_LAUNCH 5
 /* Shared runs on the tcgen05 / TMEM kernel (tensor memory accumulators, tcgen05.mma fed by descriptor from the
  * staged tiles): 0 never, 1 (default) when walking the step's wide runs (more than 32 rows) with mma.sync would
@@ -676,6 +676,9 @@ typedef struct ca_draft_args {
     const int32_t* work;        /* device: the plan's array                           */
     const ca_draft_plan_info* info;
     float* partials;            /* device scratch of ca_draft_partial_floats floats   */
+    int32_t settled;            /* 0: work and seen are read when all work before on the stream is complete, whatever wrote them.  Not 0: they came by
+                                   copies (on this stream, or on one that it has waited for), or all that wrote them has completed: the kernels may read
+                                   them while the kernel before still runs */
 } ca_draft_args;
 CA_API int64_t ca_draft_partial_floats(const ca_context* ctx, const ca_draft_plan_info* info);
 CA_API int ca_draft_attention(ca_context* ctx, const ca_draft_args* args, ca_stream stream);

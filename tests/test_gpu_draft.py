@@ -1,4 +1,5 @@
 """Attention of drafted trees over the cache, the acceptance of drafted tokens and log probabilities, against plain 64-bit forms."""
+import ctypes as C
 import math
 import random
 
@@ -273,6 +274,99 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="capacity"):
         c.cache.extend_kv([0], [[1] * 10 ** 6], k[:1].expand(10 ** 6, 2, 64), v[:1].expand(10 ** 6, 2, 64))
     c.check()
+
+
+# ---- the C entry ---------------------------------------------------------------------------------------------------------------
+class DraftArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v")] + [(n, C.c_int64) for n in ("q_node", "q_head", "k_node", "k_head", "v_node", "v_head")] + \
+        [("out", C.c_void_p), ("seen", C.c_void_p), ("words", C.c_int32), ("work", C.c_void_p), ("info", C.c_void_p), ("partials", C.c_void_p), ("settled", C.c_int32)]
+
+
+class CDraft:
+    """Trees over a context of the C library, every operand in the caller's hands."""
+
+    def __init__(self, dtype, d, own, nodes, heads=2, chunk=64, reach=4):
+        from chunk_attn import PrefixTree, cabi
+        self.cabi, lib = cabi, cabi.lib
+        g = torch.Generator(device=DEV).manual_seed(0)
+        rng = random.Random(0)
+        n_chunks = sum(n // chunk + 2 for n in own)
+        kind = cabi.CA_DTYPE_F32 if dtype == F32 else cabi.CA_DTYPE_F16
+        tree = PrefixTree(chunk, n_chunks, True)
+        pool = torch.zeros(n_chunks * heads * 2 * chunk * d * (4 if dtype == F32 else 2), dtype=torch.uint8, device=DEV)
+        self.ctx = cabi.Context(heads, d, chunk, kind, pool, n_chunks)
+
+        def normal(*shape, scale=1.0):
+            return torch.randn(shape, generator=g, device=DEV).mul_(scale).to(dtype)
+
+        self.k, self.v = [], []
+        for i, n in enumerate(own):
+            k, v = normal(n, heads, d), normal(n, heads, d)
+            row = tree.add_seq([10 ** 5 * (i + 1) + j for j in range(n)])
+            mine = [c[0] for c in tree.get_chunks() if c[1] and c[2] <= row < c[3]]
+            self.ctx.scatter_prefill(k, v, 0, n, mine)
+            self.k.insert(row, k)
+            self.v.insert(row, v)
+        self.trees = [D.random_tree(rng, n, reach) for n in nodes]
+        N = sum(nodes)
+        self.qd, self.kd, self.vd = normal(N, heads, d, scale=2.0), normal(N, heads, d), normal(N, heads, d)
+        infos, n_infos = cabi.make_infos(tree.get_chunks())
+        first = [0]
+        for n in nodes:
+            first.append(first[-1] + n)
+        plan, data = C.c_void_p(), C.POINTER(C.c_int32)()
+        self.info = cabi.DraftPlanInfo()
+        cabi.check(lib.ca_draft_plan_for_context(self.ctx._h, C.byref(plan), infos, n_infos, (C.c_int32 * len(first))(*first), len(nodes)))
+        cabi.check(lib.ca_draft_plan_data(plan, C.byref(data), C.byref(self.info)))
+        self.work = torch.tensor(data[:self.info.n_data], dtype=torch.int32)
+        lib.ca_draft_plan_destroy(plan)
+        self.seen = torch.tensor([[sum(1 << j for j in line), 0] for t in self.trees for line in D.lines(t)], dtype=torch.int32)
+        lib.ca_draft_partial_floats.restype = C.c_int64
+        floats = lib.ca_draft_partial_floats(self.ctx._h, C.byref(self.info))
+        self.partials = torch.full((max(4, floats),), math.nan, device=DEV)
+        self.scale, self.dk, self.dtype = d ** -0.5, d, dtype
+
+    def run(self, work, seen, settled=0):
+        q, k, v = self.qd, self.kd, self.vd
+        out = torch.full(q.shape, math.nan, dtype=q.dtype, device=DEV)
+        a = DraftArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_node=q.stride(0), q_head=q.stride(1), k_node=k.stride(0), k_head=k.stride(1),
+                      v_node=v.stride(0), v_head=v.stride(1), out=out.data_ptr(), seen=seen.data_ptr(), words=2, work=work.data_ptr(), info=C.addressof(self.info),
+                      partials=self.partials.data_ptr(), settled=settled)
+        self.cabi.check(self.cabi.lib.ca_draft_attention(self.ctx._h, C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        return out
+
+    def want(self):
+        return D.tree_attention(self.qd, self.kd, self.vd, self.trees, self.k, self.v, self.scale, False)
+
+
+C_SHAPES = [  # an even number of nodes: the bits must be 8-byte aligned
+    (F16, 64, (700, 30), (12, 6)), (F16, 128, (90, 64, 10), (10, 2, 12)), (F16, 80, (700, 30), (12, 6)), (F16, 80, (300,), (4,)), (F32, 64, (700, 30), (12, 6)), (F32, 128, (65, 5), (3, 1)),
+]
+
+
+@pytest.mark.parametrize("dtype,d,own,nodes", C_SHAPES)
+def test_lists_that_a_kernel_writes_right_before(dtype, d, own, nodes):
+    """The bits of the trees' lines and the work list are written by kernels ahead of the call, one of which lets its successor start early
+    (token_log_probs: the best two ids of a row of logits are a node's bits and 0)."""
+    from chunk_attn import ops
+    c = CDraft(dtype, d, own, nodes)
+    want = c.want()
+    tol = D.Case.tolerance(c, want)
+    logits = torch.zeros(len(c.seen), 1 << 13, device=DEV, dtype=F16)
+    logits[torch.arange(len(c.seen)), c.seen[:, 0].long()] = 2.0
+    logits[:, 0] = 1.0
+    work, seen = c.work.to(DEV), c.seen.to(DEV)
+    settled = c.run(work, seen, 1)
+    assert ((settled.double() - want).abs() <= tol).all()
+    for _ in range(20):
+        # bits by a kernel that its successor may overtake
+        assert torch.equal(c.run(work, ops.token_log_probs(logits, top=2)[3]), settled)
+        # both by ordinary kernels, on memory that held something else
+        late_seen, late = torch.zeros_like(seen), torch.zeros_like(work)
+        torch.add(seen, 0, out=late_seen)
+        torch.add(work, 0, out=late)
+        assert torch.equal(c.run(late, late_seen), settled)
+    assert c.ctx.status() == 0
 
 
 # ---- acceptance --------------------------------------------------------------------------------------------------------------
