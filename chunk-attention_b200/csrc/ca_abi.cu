@@ -1846,6 +1846,7 @@ int ca_draft_attention(ca_context* c, const ca_draft_args* a, ca_stream stream_)
     p.merge_off = a->work + a->info->at_off;
     p.merge_slots = a->work + a->info->at_slots;
     p.n_merge = a->info->n_merge;
+    p.n_merge_slots = (int)(a->info->n_data - a->info->at_slots);
     p.n_list = (int)((a->info->at_nodes - a->info->at_tiles) / 2);
     p.n_slots = a->info->n_slots;
     p.max_chunks = (int)c->max_chunks;

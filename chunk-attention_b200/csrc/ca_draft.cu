@@ -889,15 +889,22 @@ __global__ void __launch_bounds__(128) draft_merge_kernel(const DraftParams p) {
     if (pair >= p.n_merge * H) return;
     draft_lists_wait(p);
     const int i = pair / H, head = pair % H;
-    const int node = p.merge_nodes[i], b = p.merge_off[i], n = p.merge_off[i + 1] - b;
+    const int node = p.merge_nodes[i], b = p.merge_off[i], end = p.merge_off[i + 1];
+    const bool there = (unsigned)node < (unsigned)p.n_nodes && b >= 0 && b <= end && end <= p.n_merge_slots;
+    const int n = there ? end - b : 0;
     int slot = lane < n ? p.merge_slots[b + lane] : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    auto bad = [&] {
+        if (lane == 0) atomicCAS(p.status, STATUS_OK, STATUS_BAD_WORK_LIST);
+    };
+    if (!there) return bad();
     float M = p.sink ? 0.f : G_NEG_BIG, total = 0.f, o[COLS * 4];
 #pragma unroll
     for (int c = 0; c < COLS * 4; c++) o[c] = 0.f;
     for (int s0 = 0; s0 < n; s0 += 32) {
         if (s0 > 0) slot = s0 + lane < n ? p.merge_slots[b + s0 + lane] : 0;
+        if (__any_sync(0xffffffffu, (unsigned)slot >= (unsigned)p.n_slots)) return bad();
         const int here = min(32, n - s0);
         const int64_t at = (int64_t)slot * H + head;
         const float2 ml = lane < here ? p.part_ml[at] : make_float2(G_NEG_BIG, 0.f);

@@ -75,7 +75,7 @@ struct DraftParams {
     float2* part_ml;           // [n_slots][heads]: running maximum (log2 units), sum
     int part_width;
     const int32_t *merge_nodes, *merge_off, *merge_slots;
-    int n_merge;
+    int n_merge, n_merge_slots;
     int n_list, n_slots;       // entries of tiles, partial slots
     int max_chunks;
     int* status;

@@ -369,6 +369,26 @@ def test_lists_that_a_kernel_writes_right_before(dtype, d, own, nodes):
     assert c.ctx.status() == 0
 
 
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (F16, 80), (F32, 64)])
+def test_damaged_work_lists_are_reported(dtype, d):
+    """No entry of a work list is followed out of range: the status says that one was wrong, and the next call is right again."""
+    c = CDraft(dtype, d, (700, 700), (12, 6))
+    work, seen = c.work.to(DEV), c.seen.to(DEV)
+    want = c.run(work, seen)
+    assert c.ctx.status() == 0 and c.info.n_merge == 18
+    damage = [(w + at, x) for w, at, xs in ((0, 0, (-1, 18, 10 ** 9)), (0, 1, (0, -5, 10 ** 9)), (0, 2, (-1, 10 ** 9)), (0, 4, (10 ** 9,)), (0, 5, (-1, 10 ** 9)), (0, 6, (10 ** 9,)),
+                                            (c.info.at_nodes, 3, (-1, 18, 10 ** 9)), (c.info.at_off, 2, (-1, 10 ** 9, -2 ** 31)), (c.info.at_slots, 1, (-1, c.info.n_slots, 2 ** 31 - 1)))
+              for x in xs]
+    for at, x in damage:
+        hurt = c.work.clone()
+        hurt[at] = x
+        c.run(hurt.to(DEV), seen)
+        code, status = c.ctx.status_raw()
+        assert status == c.cabi.STATUS_BAD_WORK_LIST, (at, x)
+        c.ctx.status_clear()
+        assert torch.equal(c.run(work, seen), want) and c.ctx.status() == 0
+
+
 # ---- acceptance --------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("seed", range(4))
 @pytest.mark.parametrize("thresholds", [None, (0.09, 0.3), (0.5, 0.7)])
