@@ -608,12 +608,6 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_pairs(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], Tf32Pair b0, Tf32Pair b1) {
-    mma_tf32(d, al, b0.hi, b1.hi);
-    mma_tf32(d, ah, b0.lo, b1.lo);
-    mma_tf32(d, ah, b0.hi, b1.hi);
-}
-
 template <int D, int MT>  // head size; tiles of 16 rows
 __global__ void __launch_bounds__(G_THREADS, MT == 1 && D == 128 ? 1 : 2) draft_tf32_kernel(const __grid_constant__ DraftParams p, const GenericSizes z) {
     extern __shared__ __align__(128) uint8_t raw[];
@@ -696,48 +690,66 @@ __global__ void __launch_bounds__(G_THREADS, MT == 1 && D == 128 ? 1 : 2) draft_
                 see[h] = at.n == 32 ? 0xffffffffu : (1u << at.n) - 1;
                 if (at.chunk < 0) see[h] &= list_load(line[h] + at.first / 32);
             }
-            // few rows: one tile of scores a warp, so six sums of it, as a chain of products is what takes time
-            constexpr int SUMS = MT == 1 ? 6 : 1;
-            float s[NT][4], sums[SUMS][NT][4];
+            // Scores: products of the large parts in sums of four steps, which fp32 additions join (the tensor cores cut what they add, always towards zero);
+            // those with a small part are 2^-11 of them and stay in their own.  Few rows: one tile of scores a warp, so twice as many sums of it, as
+            // a chain of products is what takes time.
+            constexpr int CHAINS = MT == 1 ? 2 : 1, STEPS = 4 * CHAINS;
+            float s[NT][4], small[2 * CHAINS][NT][4];
 #pragma unroll
-            for (int c = 0; c < SUMS; c++)
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) sums[c][n][k] = 0.f;
-#pragma unroll(MT == 1 && D == 128 ? 8 : 4)
-            for (int ks = 0; ks < D / 8; ks++) {
-                uint32_t ah[4], al[4];
+            for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const int e = (row0 + oct + 8 * (k & 1)) * QP + 8 * ks + quad + 4 * (k >> 1);
-                    if constexpr (SPLIT) {
-                        const uint2 a = reinterpret_cast<const uint2*>(sq)[e];
-                        ah[k] = a.x;
-                        al[k] = a.y;
-                    } else {
-                        const Tf32Pair a = split_tf32(sq[e]);
-                        ah[k] = a.hi;
-                        al[k] = a.lo;
+                    s[n][k] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 2 * CHAINS; c++) small[c][n][k] = 0.f;
+                }
+#pragma unroll(MT == 1 || D == 64 ? 2 : 1)
+            for (int k0 = 0; k0 < D / 8; k0 += STEPS) {
+                float large[CHAINS][NT][4];
+#pragma unroll
+                for (int c = 0; c < CHAINS; c++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) large[c][n][k] = 0.f;
+#pragma unroll
+                for (int j = 0; j < STEPS; j++) {
+                    const int ks = k0 + j, c = j % CHAINS;
+                    uint32_t ah[4], al[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int e = (row0 + oct + 8 * (k & 1)) * QP + 8 * ks + quad + 4 * (k >> 1);
+                        if constexpr (SPLIT) {
+                            const uint2 a = reinterpret_cast<const uint2*>(sq)[e];
+                            ah[k] = a.x;
+                            al[k] = a.y;
+                        } else {
+                            const Tf32Pair a = split_tf32(sq[e]);
+                            ah[k] = a.hi;
+                            al[k] = a.lo;
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const int t = tok0 + 8 * n + oct;
+                        const float b0 = *reinterpret_cast<const float*>(sk + staged(t, 2 * ks, 0, 7) + 4 * quad), b1 = *reinterpret_cast<const float*>(sk + staged(t, 2 * ks + 1, 0, 7) + 4 * quad);
+                        const Tf32Pair p0 = split_tf32(b0), p1 = split_tf32(b1);
+                        mma_tf32(small[2 * c][n], al, p0.hi, p1.hi);
+                        mma_tf32(small[2 * c + CHAINS - 1][n], ah, p0.lo, p1.lo);
+                        mma_tf32(large[c][n], ah, p0.hi, p1.hi);
                     }
                 }
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const int t = tok0 + 8 * n + oct;
-                    const float b0 = *reinterpret_cast<const float*>(sk + staged(t, 2 * ks, 0, 7) + 4 * quad), b1 = *reinterpret_cast<const float*>(sk + staged(t, 2 * ks + 1, 0, 7) + 4 * quad);
-                    const Tf32Pair p0 = split_tf32(b0), p1 = split_tf32(b1);
-                    const int c = SUMS == 6 ? 3 * (ks & 1) : 0;
-                    mma_tf32(sums[c][n], al, p0.hi, p1.hi);
-                    mma_tf32(sums[SUMS == 6 ? c + 1 : 0][n], ah, p0.lo, p1.lo);
-                    mma_tf32(sums[SUMS == 6 ? c + 2 : 0][n], ah, p0.hi, p1.hi);
-                }
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) s[n][k] += CHAINS == 2 ? large[0][n][k] + large[CHAINS - 1][n][k] : large[0][n][k];
             }
             float high[2] = {G_NEG_BIG, G_NEG_BIG};
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    s[n][k] = SUMS == 6 ? ((sums[0][n][k] + sums[SUMS / 2][n][k]) + (sums[SUMS / 6][n][k] + sums[SUMS * 4 / 6][n][k])) + (sums[SUMS / 3][n][k] + sums[SUMS * 5 / 6][n][k]) : sums[0][n][k];
+                    s[n][k] += CHAINS == 2 ? (small[0][n][k] + small[1][n][k]) + (small[2 * CHAINS - 2][n][k] + small[2 * CHAINS - 1][n][k]) : small[0][n][k];
                     s[n][k] = (see[k >> 1] >> (tok0 + 8 * n + 2 * quad + (k & 1))) & 1 ? s[n][k] * p.scale_log2 : -INFINITY;
                     high[k >> 1] = fmaxf(high[k >> 1], s[n][k]);
                 }
@@ -758,30 +770,36 @@ __global__ void __launch_bounds__(G_THREADS, MT == 1 && D == 128 ? 1 : 2) draft_
                     s[n][k] = exp2_approx(s[n][k] - m[k >> 1]);
                     l[k >> 1] += s[n][k];  // this lane's columns only: summed over the quad at the end
                 }
-            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+            // The tile's part of the output in a sum of its own, small products first, which one fp32 operation adds: over the tokens of a long context the
+            // cuts of one running sum would add up (64 rows of 16000 tokens: 4.4e-6 off)
+            uint32_t ah[NT][4], al[NT][4];
 #pragma unroll
-                for (int i = 0; i < D / 8; i++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) o[i][k] *= alpha[k >> 1];
-            }
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                uint32_t ah[4], al[4];
+            for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) {  // A: row oct | oct + 8 of columns quad, then of quad + 4
                     const Tf32Pair a = split_tf32(s[n][2 * (k & 1) + (k >> 1)]);
-                    ah[k] = a.hi;
-                    al[k] = a.lo;
+                    ah[n][k] = a.hi;
+                    al[n][k] = a.lo;
                 }
-                // values behind the tile's tokens are anything: zero
-                const int t = tok0 + 8 * n + 2 * quad;
-                const bool on0 = t < at.n, on1 = t + 1 < at.n;
 #pragma unroll
-                for (int i = 0; i < D / 8; i++) {
-                    const int c = 8 * i + oct;
-                    const float b0 = *reinterpret_cast<const float*>(sv + staged(t, c >> 2, 0, 7) + 4 * (c & 3)), b1 = *reinterpret_cast<const float*>(sv + staged(t + 1, c >> 2, 0, 7) + 4 * (c & 3));
-                    mma_pairs(o[i], ah, al, split_tf32(on0 ? b0 : 0.f), split_tf32(on1 ? b1 : 0.f));
+            for (int i = 0; i < D / 8; i++) {
+                const int c = 8 * i + oct;
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                Tf32Pair b0[NT], b1[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    // values behind the tile's tokens are anything: zero
+                    const int t = tok0 + 8 * n + 2 * quad;
+                    const float v0 = *reinterpret_cast<const float*>(sv + staged(t, c >> 2, 0, 7) + 4 * (c & 3)), v1 = *reinterpret_cast<const float*>(sv + staged(t + 1, c >> 2, 0, 7) + 4 * (c & 3));
+                    b0[n] = split_tf32(t < at.n ? v0 : 0.f);
+                    b1[n] = split_tf32(t + 1 < at.n ? v1 : 0.f);
+                    mma_tf32(part, al[n], b0[n].hi, b1[n].hi);
+                    mma_tf32(part, ah[n], b0[n].lo, b1[n].lo);
                 }
+#pragma unroll
+                for (int n = 0; n < NT; n++) mma_tf32(part, ah[n], b0[n].hi, b1[n].hi);
+#pragma unroll
+                for (int k = 0; k < 4; k++) o[i][k] = fmaf(o[i][k], alpha[k >> 1], part[k]);
             }
         }
 #pragma unroll

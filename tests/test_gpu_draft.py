@@ -276,6 +276,18 @@ def test_refusals():
     c.check()
 
 
+@pytest.mark.parametrize("d,group,nodes", [(64, 1, 4), (64, 1, 12), (64, 1, 30), (64, 4, 64), (128, 1, 8), (128, 1, 12), (128, 1, 30), (128, 4, 64), (80, 4, 30)])
+def test_fp32_errors_do_not_grow_with_the_context(d, group, nodes):
+    """fp32 operands give fp32 results, whichever kernel multiplies them.  In the 2-norm: a product of two operands is off by 2^-22 of itself at most, so a score
+    by 2^-22 |q o k| scale = 2^-22 spread; its sums are rounded some 2^-23 of the score a group, 2^-21 spread together; a weight's
+    exponential 2^-22, the second product, its sums and the combination of pieces 2^-20 with it.  No term goes by the number of tokens."""
+    for own, spread in (((2,), 2.0), ((300, 90), 2.0), ((16000,), 2.0), ((64000,), 1.0), ((4000, 700), 8.0)):
+        c = D.Case(17, F32, 2, group, d, own=own, nodes=(nodes,) * len(own), spread=spread)
+        want = c.expected()
+        err = ((c.run().double() - want).norm() / want.norm()).item()
+        assert err <= 2.0 ** -21 * spread + 2.0 ** -20, (own, spread, err)
+
+
 # ---- the C entry ---------------------------------------------------------------------------------------------------------------
 class DraftArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v")] + [(n, C.c_int64) for n in ("q_node", "q_head", "k_node", "k_head", "v_node", "v_head")] + \
