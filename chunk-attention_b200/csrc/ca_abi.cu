@@ -1913,8 +1913,10 @@ int ca_accept_draft(const ca_accept_args* a, ca_stream stream) {
 // ---- log probabilities ---------------------------------------------------------------------------------------------------------
 int64_t ca_log_probs_scratch(int n_rows, int vocab, int dtype, int top) {
     if (n_rows < 0 || vocab < 1 || top < 0 || top > CA_MAX_TOP || !shaped_esize_of(dtype)) return -1;
-    const bool stretches = ca::log_probs_splits(n_rows, vocab, shaped_esize_of(dtype)) == 0;
-    return (int64_t)n_rows * sizeof(double2) + (stretches ? ((int64_t)n_rows + ca::log_probs_ctas()) * (int64_t)sizeof(ca::LogProbsPart) : 0);
+    const int esize = shaped_esize_of(dtype);
+    const bool stretches = ca::log_probs_splits(n_rows, vocab, esize) == 0;
+    const int64_t part = sizeof(ca::LogProbsPart) + (top > 0 ? ca::log_probs_hits_room(vocab, esize) * (int64_t)sizeof(uint32_t) : 0);
+    return (int64_t)n_rows * sizeof(double2) + (stretches ? ((int64_t)n_rows + ca::log_probs_ctas()) * part : 0);
 }
 
 int ca_token_log_probs(const ca_log_probs_args* a, ca_stream stream) {
@@ -1948,6 +1950,7 @@ int ca_token_log_probs(const ca_log_probs_args* a, ca_stream stream) {
     p.top_ids = a->top_ids;
     p.lse = static_cast<double2*>(a->scratch);
     p.parts = reinterpret_cast<ca::LogProbsPart*>(p.lse + a->n_rows);
+    p.hits = reinterpret_cast<uint32_t*>(p.parts + (int64_t)a->n_rows + ca::log_probs_ctas());
     p.tokens_here = a->n_rows > 0 && (!a->rows || a->n_tokens <= 1024);  // every row's CTA reads the rows of all tokens
     CA_CUDA(ca::launch_log_probs(p, a->dtype, static_cast<cudaStream_t>(stream)));
     return CA_OK;

@@ -581,7 +581,8 @@ __global__ void __launch_bounds__(L_THREADS, 4) log_probs_kernel(const LogProbsP
                         to.n_hits = hits;
                     }
                 }
-                for (int i = tid; i < min(hits, L_HITS); i += L_THREADS) to.hits[i] = sh.hits[place][i];
+                uint32_t* const notes = p.hits + ((int64_t)s.row + blockIdx.x) * p.hits_room;
+                for (int i = tid; i < min(hits, p.hits_room); i += L_THREADS) notes[i] = sh.hits[place][i];
             }
             turn_at = ((int64_t)s.row + 1) * p.turns;
             if (turn_at >= turn_end) {
@@ -695,7 +696,7 @@ __global__ void __launch_bounds__(F_THREADS) finish_rows_kernel(const LogProbsPa
         const Stat one = {from.m, from.l, from.a};
         if (TOP) {
             limit = fmaxf(limit, from.limit);
-            many = many || from.n_hits > L_HITS;
+            many = many || from.n_hits > p.hits_room;
         }
         st = join(st, one);
     }
@@ -708,7 +709,7 @@ __global__ void __launch_bounds__(F_THREADS) finish_rows_kernel(const LogProbsPa
         if (!many)
             for (int b = b0; b <= b1; b++) {
                 const LogProbsPart& from = p.parts[(int64_t)row + b];
-                look_at(s.x + s.head, s.head, min(s.n_vec, (int)max((int64_t)0, p.begin(b) - row_begin) * L_STEP), from.hits, from.n_hits, limit, tid, F_THREADS, keep);
+                look_at(s.x + s.head, s.head, min(s.n_vec, (int)max((int64_t)0, p.begin(b) - row_begin) * L_STEP), p.hits + ((int64_t)row + b) * p.hits_room, from.n_hits, limit, tid, F_THREADS, keep);
             }
         const int around = s.head + (p.vocab - s.head - s.n_vec * Vec<T>::N);  // logits outside of whole vectors
         if (tid < around) {
@@ -788,7 +789,11 @@ int log_probs_splits(int n_rows, int vocab, int esize) {
     return s;
 }
 
+// A note is of one whole vector at least: short rows cannot have more of them
+int log_probs_hits_room(int vocab, int esize) { return std::min(L_HITS, std::max(1, vocab / (16 / esize))); }
+
 void log_probs_shape(LogProbsParams& p, int esize) {
+    p.hits_room = log_probs_hits_room(p.vocab, esize);
     p.splits = log_probs_splits(p.n_rows, p.vocab, esize);
     p.turns = turns_of(p.vocab, esize);
     const int64_t all = (int64_t)p.n_rows * p.turns;

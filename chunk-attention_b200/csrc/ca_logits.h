@@ -9,8 +9,7 @@ constexpr int LOG_PROBS_HITS = 512;
 struct LogProbsPart {  // what a stretch of a row gives
     float m, l, a;     // reference (log2 units), sum, sum of y 2^y
     float limit;       // threshold of the best
-    int n_hits;
-    uint32_t hits[LOG_PROBS_HITS];  // notes of vectors that reached it
+    int n_hits;        // notes of vectors that reached it
 };
 struct LogProbsParams {
     const void* logits;      // [n_rows, vocab]
@@ -28,6 +27,8 @@ struct LogProbsParams {
     float* top_log_probs;    // [n_rows, top]
     int32_t* top_ids;
     LogProbsPart* parts;     // [n_rows + log_probs_ctas()], when stretches are handed out
+    uint32_t* hits;          // [n_rows + log_probs_ctas()][hits_room]: their notes, where the best are asked for
+    int hits_room;
     double2* lse;            // [n_rows]: a reference, log of the sum relative to it
     bool tokens_here;        // the rows' CTAs look the tokens up, else a kernel behind them does
 #if defined(__CUDACC__)
@@ -40,6 +41,7 @@ struct LogProbsParams {
 };
 int log_probs_splits(int n_rows, int vocab, int esize);
 int log_probs_ctas();        // that share all rows
+int log_probs_hits_room(int vocab, int esize);
 void log_probs_shape(LogProbsParams& p, int esize);  // splits and turns, from n_rows and vocab
 cudaError_t read_log_probs_status(int* status, cudaStream_t stream);  // 0, or STATUS_* of the first wait that ran out
 cudaError_t launch_log_probs(const LogProbsParams& p, int dtype, cudaStream_t stream);

@@ -183,3 +183,12 @@ def test_log_probs_without_rows_take_a_token_for_every_row():
     ok.update(row_stride=100, n_rows=4, vocab=100, dtype=cabi.CA_DTYPE_F32, n_tokens=4, top=3, rows=0)
     for change in ({"n_tokens": 3}, {"n_tokens": 5}, {"n_rows": 0}, {"n_tokens": 1, "top": 0}):
         refused(cabi.lib.ca_token_log_probs, LogProbsArgs(**dict(ok, **change)), "one token per row")
+
+
+def test_log_probs_scratch_goes_by_what_is_asked():
+    """A row's part without the best tokens is a few numbers; notes of the best are no more than the row has vectors."""
+    size = cabi.lib.ca_log_probs_scratch
+    assert size(1 << 20, 100, cabi.CA_DTYPE_F16, 0) < 64 * (1 << 20)
+    assert size(1 << 20, 100, cabi.CA_DTYPE_F16, 5) < 128 * (1 << 20)  # 200 bytes of logits a row
+    assert size(131072, 32000, cabi.CA_DTYPE_F16, 0) < 64 * 131072 < size(131072, 32000, cabi.CA_DTYPE_F16, 1) < 4096 * 131072
+    assert size(1 << 20, 3, cabi.CA_DTYPE_BF16, 3) > 0

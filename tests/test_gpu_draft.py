@@ -595,6 +595,18 @@ def test_log_probs_do_not_go_by_the_size_of_logits(n, vocab, top):
         check_log_probs_closely((x + offset).bfloat16(), top)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("vocab", [1, 3, 8, 9, 100, 1024, 4100])
+def test_log_probs_of_short_rows_by_the_thousands(dtype, vocab):
+    """More notes than a short row has vectors need no room: rising, equal and falling logits, rows that start at any address."""
+    n, top = 3000, min(vocab, 7)
+    x = torch.randn(n, vocab + 1, device=DEV, generator=torch.Generator(DEV).manual_seed(8)) * 3
+    x[::3] = x[::3].sort(-1).values
+    x[1::3, :] = 0.5
+    check_log_probs_closely(x.to(dtype)[:, 1:], top)
+    check_log_probs_closely(x.to(dtype)[:, :vocab].contiguous(), 0)
+
+
 def test_log_probs_of_named_tokens():
     from chunk_attn import ops
     x = torch.randn(4, 100, device=DEV)
