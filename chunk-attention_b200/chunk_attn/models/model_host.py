@@ -23,7 +23,7 @@ from .sequence import Sequence
 class ModelHost:
     def __init__(self, model_obj, kv_caches, max_batch_size=32, draft=None, thresholds=None):
         """draft(tokens, depth) -> (drafted tokens, parents): decode steps check drafted tokens, for models with
-        `decode_drafts`; thresholds as there."""
+        `decode_drafts`; thresholds as there.  A draft with `follow()` gives every sequence a drafter of its own."""
         if draft is not None and not hasattr(model_obj, "decode_drafts"):
             raise ValueError("%s does not decode drafted tokens" % type(model_obj).__name__)
         self.model_obj = model_obj
@@ -127,7 +127,10 @@ class ModelHost:
         """One decode step over drafted tokens.  The draft is asked for lines that end with the sequence; what a longer one brings
         beyond its end is dropped."""
         seqs = self.running_seqs
-        drafts = [self.draft(s.tokens, s.max_tokens + len(s.prompt_tokens) - len(s) - 1) for s in seqs]
+        for s in seqs:
+            if s.drafter is None:
+                s.drafter = self.draft.follow() if hasattr(self.draft, "follow") else self.draft
+        drafts = [s.drafter(s.tokens, s.max_tokens + len(s.prompt_tokens) - len(s) - 1) for s in seqs]
         top = max((s.log_probs for s in seqs if s.log_probs is not None), default=0)
         new, told = self.model_obj.decode_drafts(seqs, self.kv_caches, drafts, self.thresholds, top)
         for seq, (drafted, _), tokens, about in zip(seqs, drafts, new, told):

@@ -18,6 +18,7 @@ class Sequence:
         self.tokens = list(self.prompt_tokens)
         self.log_probs = log_probs
         self.token_log_probs = []
+        self.drafter = None  # set by a host that decodes drafted tokens
         self.index = None
         self.error = None
         self.result_ready = threading.Event()

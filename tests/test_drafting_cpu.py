@@ -39,6 +39,78 @@ def test_drafts_are_trees_of_the_text():
         assert max(deep, default=0) <= depth
 
 
+def scan(look, tokens, depth):
+    """The definition: the latest places after the longest ending that stood before."""
+    for n in range(min(look.ngram, len(tokens) - 1), 0, -1):
+        places = [i + n for i in range(len(tokens) - n - 1, -1, -1) if tokens[i:i + n] == tokens[-n:]][:look.lines]
+        if places and depth > 0:
+            return look._tree([tokens[i:i + depth] for i in places])
+    return [], []
+
+
+def test_followers_draft_what_the_text_says():
+    rng = random.Random(2)
+    for _ in range(100):
+        look = PromptLookup(rng.randint(1, 9), rng.randint(1, 4), rng.randint(1, 3))
+        follower, tokens, words = look.follow(), [], rng.randint(1, 6)
+        for _ in range(rng.randint(1, 30)):
+            tokens += [rng.randrange(words) for _ in range(rng.randint(0, 4))]
+            depth = rng.randint(0, 6)
+            want = scan(look, tokens, depth)
+            assert look(tokens, depth) == want
+            assert follower(tokens, depth) == want
+    follower = look.follow()
+    follower([1, 2, 3], 4)
+    with pytest.raises(ValueError, match="shorter"):
+        follower([1, 2], 4)
+
+
+class Counted(list):
+    """Counts the elements that are read."""
+    read = 0
+
+    def __getitem__(self, i):
+        x = super().__getitem__(i)
+        Counted.read += len(x) if isinstance(i, slice) else 1
+        return x
+
+
+def test_a_draft_does_not_go_through_the_text_again():
+    look = PromptLookup(8)
+    tokens = Counted(range(16000))
+    Counted.read = 0
+    assert look(tokens, 8) == ([], [])
+    assert Counted.read < 2 * 16000  # a call by itself: once
+    follower = look.follow()
+    follower(tokens, 8)
+    Counted.read = 0
+    for i in range(10):
+        tokens.append(20000 + i)
+        assert follower(tokens, 8) == ([], [])
+    assert Counted.read < 10 * 32
+
+
+def test_the_host_gives_every_sequence_a_drafter():
+    look, made = PromptLookup(4), []
+
+    class Source:
+        def __call__(self, tokens, depth):
+            raise AssertionError("the followers draft")
+
+        def follow(self):
+            made.append(look.follow())
+            return made[-1]
+
+    host = ModelHost(DraftingModel(), [H.TreeCache()], max_batch_size=2, draft=Source())
+    host.cycle_time = 0.02
+    prompts = [[1, 2, 3, 1, 2], [4, 4, 4], [5, 6]]
+    with host:
+        seqs = [host.predict_async(p, 20) for p in prompts]
+        for seq, p in zip(seqs, prompts):
+            assert seq.get_result(timeout=60) == H.rollout(p, 20)
+    assert len(made) == 3
+
+
 class DraftingModel(H.TreeModel):
     """Takes drafted tokens as the decoder does: the longest line that its own next tokens agree with."""
 
