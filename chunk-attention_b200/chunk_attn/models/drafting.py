@@ -6,6 +6,23 @@ follow, a lower one, or -1 for the sequence's last token.  The model attends to 
 """
 
 
+def cut(draft, depth):
+    """The draft without what stands deeper than `depth` tokens."""
+    tokens, parents = draft
+    if len(tokens) != len(parents):
+        raise ValueError("one parent per drafted token is required")
+    deep, at, kept = [], {-1: -1}, ([], [])  # at: the new numbers of those that stay
+    for i, (token, p) in enumerate(zip(tokens, parents)):
+        if not -1 <= p < i:
+            raise ValueError("a drafted token's parent must be a token before it, or -1")
+        deep.append(1 if p < 0 else deep[p] + 1)
+        if deep[i] <= depth:
+            at[i] = len(kept[0])
+            kept[0].append(token)
+            kept[1].append(at[p])
+    return kept
+
+
 class PromptLookup:
     """Drafts from the sequence's own text: where its last tokens have stood before, what followed them is drafted.
 

@@ -17,6 +17,7 @@ import torch
 from chunk_attn import ops
 
 from ..logger import logger
+from .drafting import cut
 from .sequence import Sequence
 
 
@@ -125,12 +126,13 @@ class ModelHost:
 
     def decode_drafts(self):
         """One decode step over drafted tokens.  The draft is asked for lines that end with the sequence; what a longer one brings
-        beyond its end is dropped."""
+        beyond its end is dropped before the model sees it (it may be beyond the model's last position, too)."""
         seqs = self.running_seqs
         for s in seqs:
             if s.drafter is None:
                 s.drafter = self.draft.follow() if hasattr(self.draft, "follow") else self.draft
-        drafts = [s.drafter(s.tokens, s.max_tokens + len(s.prompt_tokens) - len(s) - 1) for s in seqs]
+        left = [s.max_tokens + len(s.prompt_tokens) - len(s) - 1 for s in seqs]
+        drafts = [cut(s.drafter(s.tokens, n), n) for s, n in zip(seqs, left)]
         top = max((s.log_probs for s in seqs if s.log_probs is not None), default=0)
         new, told = self.model_obj.decode_drafts(seqs, self.kv_caches, drafts, self.thresholds, top)
         for seq, (drafted, _), tokens, about in zip(seqs, drafts, new, told):

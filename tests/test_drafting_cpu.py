@@ -4,7 +4,7 @@ import random
 import pytest
 
 import test_model_host_cpu as H
-from chunk_attn.models.drafting import PromptLookup
+from chunk_attn.models.drafting import PromptLookup, cut
 from chunk_attn.models.model_host import ModelHost
 
 
@@ -175,3 +175,38 @@ def test_host_refuses():
     host.stopped = False
     with pytest.raises(ValueError, match="log_probs"):
         host.predict_async([1], 1, log_probs=33)
+
+
+class LimitedModel(DraftingModel):
+    """Has positions for no more than `limit` tokens, as decoders do, and refuses steps that need more."""
+    limit = 12
+
+    def decode_drafts(self, seqs, kv_caches, drafts, thresholds, top):
+        for seq, (tokens, parents) in zip(seqs, drafts):
+            deep = []
+            for p in parents:
+                deep.append(1 if p < 0 else deep[p] + 1)
+            if len(seq) - 1 + max(deep, default=0) >= self.limit:
+                raise ValueError("sequence exceeds the last position")
+        return super().decode_drafts(seqs, kv_caches, drafts, thresholds, top)
+
+
+def test_a_draft_beyond_the_last_position_does_not_fail_the_host():
+    """Requests that end at the model's last position are served whatever the draft brings beyond it."""
+    def draft(tokens, depth):
+        return H.rollout(tokens, 9)[len(tokens):] + [1, 2, 3], list(range(-1, 8)) + [-1, 9, 10]
+
+    host = ModelHost(LimitedModel(), [H.TreeCache()], max_batch_size=2, draft=draft)
+    host.cycle_time = 0.02
+    with host:
+        for n in (2, 4, 9, 10):
+            assert host.predict([4, 5, 6], n) == H.rollout([4, 5, 6], n)
+        assert host.failure is None
+
+
+def test_cut():
+    assert cut(([7, 8, 9, 5, 6], [-1, 0, 1, -1, 3]), 2) == ([7, 8, 5, 6], [-1, 0, -1, 2])
+    assert cut(([7, 8, 9], [-1, 0, 1]), 3) == ([7, 8, 9], [-1, 0, 1]) and cut(([7, 8], [-1, -1]), 0) == ([], [])
+    for bad in (([1], []), ([1], [0]), ([1, 2], [-1, -2])):
+        with pytest.raises(ValueError):
+            cut(bad, 4)
