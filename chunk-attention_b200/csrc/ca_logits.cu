@@ -11,7 +11,7 @@
 // or too many (rising or equal logits) go by insertion.
 //
 // What bounds it: instructions (an exponential and some five others a logit) at 0.6 to 0.75 of the copy rate, then the second kernel's chain of
-// dependent reads.  2048 rows of 128000 in bf16 with 20 best 131 us (floor 80), 1536 rows of 32000 in fp16 with one 34 (15), 517 rows of 50001 in fp32
+// dependent reads.  2048 rows of 128000 in bf16 with 20 best 128 us (floor 80), 1536 rows of 32000 in fp16 with one 34 (15), 517 rows of 50001 in fp32
 // with 8 30 (16); one row of 32000 in fp32 with 5 by a cluster 7.5 us.
 #include <algorithm>
 #include <cmath>
