@@ -609,6 +609,7 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
 template <int D, int MT>  // head size; tiles of 16 rows
 __global__ void __launch_bounds__(G_THREADS, MT == 1 && D == 128 ? 1 : 2) draft_tf32_kernel(const __grid_constant__ DraftParams p, const GenericSizes z) {
     extern __shared__ __align__(128) uint8_t raw[];
